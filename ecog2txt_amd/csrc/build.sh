@@ -12,7 +12,7 @@ obj="$here/build"
 dbg=()
 if [ "${E2T_DEBUG:-0}" = 1 ]; then out="$here/../libecog2txt_hip_dbg.so"; obj="$here/build_dbg"; dbg=(-DE2T_DEBUG); fi
 mkdir -p "$obj"
-srcs=(runtime gemm lstm lstm_big elementwise comm)
+srcs=(runtime gemm lstm lstm_big elementwise comm gemm_i8 sample)
 # no packed fp32 arithmetic (v_pk_add/mul/fma_f32): hipcc forms it from ordinary float code by itself, and some of its forms have
 # given wrong results on this chip now and then (hipcc's host pass warns that it does not know the feature: harmless)
 nopk=(-Xclang -target-feature -Xclang -packed-fp32-ops)

@@ -25,6 +25,7 @@ extern "C" int e2t_sizeof(int which) {
         case 4: return (int)sizeof(e2t_dropout);
         case 5: return (int)sizeof(e2t_gemm_call);
         case 6: return (int)sizeof(e2t_tile_desc);
+        case 7: return (int)sizeof(e2t_sample_cfg);
         default: return -1;
     }
 }

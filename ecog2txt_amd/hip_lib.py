@@ -69,7 +69,14 @@ class AdamHyper(C.Structure):
                 ('ema_decay', C.c_float), ('grad_scale', C.c_float), ('step_offset', C.c_int), ('skip_if_nonzero', C.c_void_p)]
 
 
+class SampleCfg(C.Structure):
+    _fields_ = [('temperature', C.c_float), ('top_p', C.c_float), ('min_p', C.c_float), ('top_k', C.c_int),
+                ('temperature_rows', C.c_void_p), ('top_k_rows', C.c_void_p), ('top_p_rows', C.c_void_p), ('min_p_rows', C.c_void_p)]
+
+
+DT_F32, DT_BF16 = 0, 1    # E2T_DT_*
 _p, _i, _f, _l, _z = C.c_void_p, C.c_int, C.c_float, C.c_long, C.c_size_t
+_ll = C.c_longlong
 
 # name -> argtypes; the list mirrors include/ecog2txt_hip.h one to one
 SIGNATURES = {
@@ -116,6 +123,11 @@ SIGNATURES = {
     'e2t_greedy_head_small': [_p, _i, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _p, _p, _p, _p, _z, _p, _p, _p],
     'e2t_beam_step': [_p, _i, _i, _i, _i, _f, _i, _i, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p, _p],
     'e2t_beam_reorder': [_p, _i, _p, _i, _i, _p, _p, _p, _p],
+    'e2t_quant_rows_i8': [_p, _i, _ll, _i, _i, _p, _ll, _p, _p],
+    'e2t_gemm_nt_i8': [_p, _ll, _p, _p, _ll, _p, _p, _p, _ll, _i, _i, _i, _i, _p],
+    'e2t_linear_i8': [_p, _i, _ll, _p, _ll, _p, _p, _p, _ll, _i, _i, _i, _i, _p, _z, _p],
+    'e2t_sample_rows': [_p, _i, _ll, _i, _i, _p, C.POINTER(SampleCfg), _p, _p, _p, _z, _p],
+    'e2t_sample_step': [_p, _i, _ll, _i, _i, _p, C.POINTER(SampleCfg), _i, _i, _i, _i, _p, _p, _p, _p, _p, _z, _p],
     'e2t_mse': [_p, _i, _p, _i, _i, _p, _i, _p, _f, _p, _p, _i, _p],
     'e2t_inc_step': [_p, _p, _p],
     'e2t_adam_ema_step': [_p, _p, _p, _p, _p, _z, _p, C.POINTER(AdamHyper), _p],
@@ -133,6 +145,7 @@ SIGNATURES = {
 COMM_ID_BYTES = 128
 PLAIN = {'e2t_abi_version': ([], C.c_int), 'e2t_sizeof': ([_i], C.c_int), 'e2t_last_error': ([], C.c_char_p), 'e2t_device_cus': ([_i], C.c_int),
          'e2t_bwd_persist_kq': ([_i], C.c_int), 'e2t_lstm_big_ok': ([_i], C.c_int), 'e2t_conv_fwd_fused_ok': ([_i, _i], C.c_int), 'e2t_comm_rank': ([_p], C.c_int), 'e2t_comm_size': ([_p], C.c_int),
+         'e2t_linear_i8_ws_bytes': ([_i, _i], C.c_size_t), 'e2t_sample_ws_bytes': ([_i, _i], C.c_size_t),
          'e2t_crc32c': ([_p, _z, C.c_uint32], C.c_uint32)}
 
 _lib = None

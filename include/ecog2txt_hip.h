@@ -38,7 +38,7 @@ extern "C" {
 
 int e2t_abi_version(void);
 /* sizeof() of the structs that cross the boundary, for bindings to check their layouts against:
- * which = 0 e2t_gemm_epilogue, 1 e2t_lstm_desc, 2 e2t_pack_desc, 3 e2t_adam_hyper, 4 e2t_dropout, 5 e2t_gemm_call, 6 e2t_tile_desc [ABI 8];
+ * which = 0 e2t_gemm_epilogue, 1 e2t_lstm_desc, 2 e2t_pack_desc, 3 e2t_adam_hyper, 4 e2t_dropout, 5 e2t_gemm_call, 6 e2t_tile_desc [ABI 8], 7 e2t_sample_cfg;
  * -1 for any other value */
 int e2t_sizeof(int which);
 const char* e2t_last_error(void);          /* thread-local, host pointer */
@@ -320,6 +320,50 @@ int e2t_beam_step(const float* logits, int ldl, int B, int W, int V, float tempe
 /* the decoder state (one direction) of the surviving hypotheses: row r of Yblk (bf16 [rows][ldy], one time block of Yext) and of
  * the step's lane-native cell save Cs_step <- those of row rowmap[r]; tmp_h bf16 [rows][roundup(H,8)], tmp_c fp32 [rows][H] */
 int e2t_beam_reorder(void* Yblk, int ldy, float* Cs_step, int rows, int H, const int32_t* rowmap, void* tmp_h, float* tmp_c, void* stream);
+/* ---- serving: the decoder's output side with 8-bit weights, and drawing words instead of taking the arg-max.  (The reference decodes
+ *      greedily or by beam in fp32: beam_width, temperature, mocha-1_word_sequence.yaml:31, 82.) ---- */
+#define E2T_DT_F32 0
+#define E2T_DT_BF16 1
+/* Rows in 8 bits: top[m] = the largest finite |x[m][k]|, scale[m] = top / 127 (fp32), q[m][k] = 127 x / top rounded to the nearest
+ * whole number, ties to even, exactly.  NaN becomes 0, +-inf +-127; a row of zeros has scale 0.  x fp32 or bf16 [M][ldx]; q [M][ldq],
+ * 16-B aligned, ldq a multiple of 16 >= K rounded up to 64: the columns from K up to that are written as zeros, nothing behind them. */
+int e2t_quant_rows_i8(const void* x, int dtype, long long ldx, int M, int K, int8_t* q, long long ldq, float* scale, void* stream);
+/* C[m][n] = sa[m] * sb[n] * sum_k A[m][k] * B[n][k] (+ bias[n]): A int8 [M][lda] (one scale a row = token), B int8 [N][ldb] (one scale a
+ * row = output channel), both 16-B aligned with leading dimensions that are multiples of 16 and >= K rounded up to 64; columns
+ * from K up to that must be zero in at least one of the two (e2t_quant_rows_i8 writes them so).  The integer sum is exact
+ * (K <= E2T_I8_MAX_K), then rounded to fp32 once; scales, bias and the optional ReLU in fp32.  flags: E2T_GEMM_RELU,
+ * E2T_GEMM_OUT_BF16 (C bf16 instead of fp32); others are refused. */
+#define E2T_I8_MAX_K 131071
+int e2t_gemm_nt_i8(const int8_t* A, long long lda, const float* sa, const int8_t* B, long long ldb, const float* sb, const float* bias,
+                   void* C, long long ldc, int M, int N, int K, int flags, void* stream);
+/* the same from activations: e2t_quant_rows_i8(x) and e2t_gemm_nt_i8 in one call.  ws: device memory of e2t_linear_i8_ws_bytes(M, K),
+ * 16-B aligned, needed until the call has run; its content does not matter. */
+size_t e2t_linear_i8_ws_bytes(int M, int K);
+int e2t_linear_i8(const void* x, int dtype, long long ldx, const int8_t* W, long long ldw, const float* sw, const float* bias, void* y,
+                  long long ldy, int M, int N, int K, int flags, void* ws, size_t ws_bytes, void* stream);
+/* One token a row from logits [B][ldl] (fp32 or bf16) and one uniform number u[b] in [0, 1).  Tokens rank by logit, equal ones by
+ * index.  Kept are, of the tokens whose logit is above -inf (NaN counts as -inf, +inf as the largest finite number): the top_k
+ * first (<= 0 or >= V: all); of those the shortest prefix whose probability reaches top_p of theirs (>= 1: all; at least one);
+ * of those the tokens with at least min_p times the largest probability (<= 0: all; above 1 counts as 1).  Drawn is the first
+ * token, by index, at which the kept probabilities' running sum exceeds u times their sum.  temperature <= 0 (or NaN) takes the
+ * first token of the ranking.  token[b] = -1 where no logit is above -inf.  logprob[b] (or NULL): the natural logarithm of the
+ * token's probability among the kept ones (0 for temperature <= 0, -inf for token -1).
+ * The answer does not depend on launch shape, order of sums or other rows: sums are of whole numbers (probability in units of
+ * 2^-F of the largest, F = min(50, 62 - ceil(log2 V))).  A settings array, where given, holds one value a row (device memory);
+ * the scalar counts where it is NULL.  ws: device memory of e2t_sample_ws_bytes(B, V), 16-B aligned, needed until the call has run. */
+#define E2T_SAMPLE_MAX_V 1048576
+typedef struct e2t_sample_cfg {
+    float temperature, top_p, min_p; int top_k;
+    const float* temperature_rows; const int32_t* top_k_rows; const float* top_p_rows; const float* min_p_rows;
+} e2t_sample_cfg;
+size_t e2t_sample_ws_bytes(int B, int V);
+int e2t_sample_rows(const void* logits, int dtype, long long ldl, int B, int V, const float* u, const e2t_sample_cfg* cfg /* host pointer */,
+                    int32_t* token, float* logprob, void* ws, size_t ws_bytes, void* stream);
+/* the same with e2t_greedy_step's bookkeeping in the launch: out[b][l] = done[b] ? pad : token, done[b] |= token == eos, next_tok[b]
+ * (or NULL) = token, score[b] (or NULL) += logprob while not done.  A row with nothing to draw from ends (token eos, score -inf). */
+int e2t_sample_step(const void* logits, int dtype, long long ldl, int B, int V, const float* u, const e2t_sample_cfg* cfg, int l, int Lmax,
+                    int eos, int pad, int32_t* done, int32_t* out, int32_t* next_tok, float* score, void* ws, size_t ws_bytes, void* stream);
+
 /* ---- a8: Gaussian encoder-target head ---- */
 int e2t_mse(const float* P, int ldp, const float* At, int M, int K, const int32_t* lens, int rows_per_step,
             const int32_t* nval, float weight, float* rowloss, void* dP, int lddp, void* stream);
