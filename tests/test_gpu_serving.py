@@ -413,7 +413,7 @@ def test_sample_step_bookkeeping():
     out = torch.full((B, L), -5, dtype=torch.int32, device='cuda')
     nxt = torch.full((B,), -5, dtype=torch.int32, device='cuda')
     score = torch.full((B,), 0.5, device='cuda')
-    cfg = S.sample_config(B, l.device, top_k=20)
+    cfg = S.sample_config(B, l.get_device(), top_k=20)
     n = H.lib.e2t_sample_ws_bytes(B, V)
     ws = torch.empty(max(n, 16), dtype=torch.uint8, device='cuda')
     H.lib.e2t_sample_step(l.data_ptr(), H.DT_F32, V, B, V, u.data_ptr(), C.byref(cfg), 2, L, eos, pad, done.data_ptr(), out.data_ptr(), nxt.data_ptr(),
