@@ -3,11 +3,19 @@
 // The mathematics.  z = l / T ranks like l itself, so every filter keeps a PREFIX of one order: value descending, index ascending.
 // That order is the ascending order of the 64-bit word  rank = (~monotone(l) << 32) | index  (unique per token), and "what is kept"
 // is  rank <= cut  (top-k and top-p) together with  z - z_max >= log(min_p).
-// Masses are WHOLE NUMBERS: w_i = round(2^F exp(z_i - z_max)), F = min(50, 62 - ceil(log2 V)), the exponential in double precision.
-// Integer sums do not depend on their order: any split of a row over threads, waves or workgroups, and any order of atomics, gives
-// the same sums, the same cut and the same token, bit for bit.  (A token below 2^-F of the largest weighs nothing: V of them
-// together are below 2^-12 of the resolution of u.)  fp32 sums would not do: over a flat vocabulary of 128 k tokens the borders
-// between tokens lie 8e-6 of the whole apart and 6e-8 of rounding moves the answer of one row in a hundred.
+// Masses are WHOLE NUMBERS: w_i = round(2^F exp(z_i - z_max)), F = min(50, 62 - ceil(log2 V)), the exponential in double precision;
+// what lies 32 or more below the maximum (e^-32 = 1.3e-14) weighs nothing.  Integer sums do not depend on their order: any split of
+// a row over threads, waves or workgroups, and any order of atomics, gives the same sums, the same cut and the same token, bit for
+// bit.  fp32 sums would not do: over a flat vocabulary of 128 k tokens the borders between tokens lie 8e-6 of the whole apart and
+// 6e-8 of rounding moves the answer of one row in a hundred.
+// fp64 multiply-adds run at the rate of unpacked fp32 ones on this chip; the exponential is a product of two table entries (LDS) and
+// a polynomial of degree 6 over 1/64.
+//
+// Finding the cut.  A histogram of 2048 bins of 1/64 in z (count and mass in one 64-bit LDS atomic) says in which bin the k-th token, or
+// p of the mass, lies; only that bin's tokens are ranked among themselves.
+//
+// Rows up to SMP_ROW_MAX tokens: one workgroup a row, the row in registers, one launch (k_sample_row).  Longer rows: four launches, the row
+// spread over many workgroups (k_sample_hist, _zone, _gather, _draw).
 #include "common.h"
 #include "ecog2txt_hip.h"
 #include <math.h>
@@ -15,9 +23,10 @@
 typedef unsigned long long u64;
 #define ST ((hipStream_t)stream)
 
-#define SMP_NT 1024                 // threads of the one-workgroup-per-row kernel
-#define SMP_BINS 2048               // level-1 histogram: bins of 1/64 in z below the maximum (window 32: e^-32 = 1.3e-14)
-#define SMP_PER_Z 64.0
+#define SMP_BINS 2048
+#define SMP_TILE 4096               // long rows: tokens of a tile (256 threads x 16)
+#define SMP_CHUNK_TILES 12          // tiles of a workgroup of k_sample_hist at most (the packed word's bits)
+#define SMP_LIST 8192               // long rows: tokens around the cut that are kept in a list
 
 struct SampleArgs {
     const void* logits; long long ldl; int V, frac;            // frac = F
@@ -25,22 +34,54 @@ struct SampleArgs {
     float t0, p0, m0; int k0;                                  // settings of all rows ...
     const float* t; const int* k; const float* p; const float* m;   // ... or [B] each
     int* token; float* logprob;
-    u64* list;                                                 // [B][V] ranks of the tokens around the cut (workspace)
     // bookkeeping of a decoder step (done == NULL: none)
     int l, Lmax, eos, pad; int *done, *out, *next_tok; float* score;
+    char* ws; int G, tiles;                                    // long rows: workspace, workgroups (chunks) and tiles a row
 };
-
-template <bool BF16> __device__ __forceinline__ float logit_at(const void* row, int i) {
-    float v = BF16 ? bf2f(((const bf16_t*)row)[i]) : ((const float*)row)[i];
-    if (!(v == v)) v = -INFINITY;                              // NaN: never drawn
-    v = fminf(v, 3.402823466e+38f);                            // +inf: the largest finite number
-    return v + 0.0f;                                           // (-0 ties with +0)
+struct Settings { float T, P, M; int k; bool use_k, use_p, use_m, greedy; };
+__device__ __forceinline__ Settings settings_of(const SampleArgs& a, int b) {
+    Settings s;
+    s.T = a.t ? a.t[b] : a.t0; s.P = a.p ? a.p[b] : a.p0; s.M = a.m ? a.m[b] : a.m0; s.k = a.k ? a.k[b] : a.k0;
+    s.use_p = s.P < 1.0f; s.use_k = s.k > 0 && s.k < a.V; s.use_m = s.M > 0.0f; s.greedy = !(s.T > 0.0f);
+    return s;
 }
+
+// ---- logits -------------------------------------------------------------------------------------------------------------------------
+// NaN is never drawn, +inf is the largest finite number, -0 ties with +0
+__device__ __forceinline__ float clean(float v) { if (!(v == v)) v = -INFINITY; return fminf(v, 3.402823466e+38f) + 0.0f; }
+// 16-byte groups of a row: group q holds elements q * E - o .. + E - 1 (E = 4 fp32, 8 bf16; o = the row's offset from a 16-byte boundary).
+// Only groups that lie wholly inside the row are loaded whole.
+template <bool BF16> struct Row {
+    static constexpr int E = BF16 ? 8 : 4;
+    const char* row; int V, o;
+    __device__ __forceinline__ Row(const SampleArgs& a, int b) {
+        row = (const char*)a.logits + (size_t)b * a.ldl * (BF16 ? 2 : 4); V = a.V;
+        o = (int)(((uintptr_t)row & 15) / (BF16 ? 2 : 4));
+    }
+    __device__ __forceinline__ float at(int i) const { return clean(BF16 ? bf2f(((const bf16_t*)row)[i]) : ((const float*)row)[i]); }
+    // E elements of group q; -inf outside the row
+    __device__ __forceinline__ void group(int q, float* v) const {
+        const int i = q * E - o;
+        if (i >= 0 && i + E <= V) {
+            const uint4 w = *(const uint4*)(row + (long long)i * (BF16 ? 2 : 4));
+            const unsigned x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (BF16) { v[2 * e] = clean(__uint_as_float(x[e] << 16)); v[2 * e + 1] = clean(__uint_as_float(x[e] & 0xFFFF0000u)); }
+                else v[e] = clean(__uint_as_float(x[e]));
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = i + e >= 0 && i + e < V ? at(i + e) : -INFINITY;
+        }
+    }
+};
 __device__ __forceinline__ unsigned mono(float v) { const unsigned b = __float_as_uint(v); return b ^ ((b >> 31) ? 0xFFFFFFFFu : 0x80000000u); }
 __device__ __forceinline__ float unmono(unsigned o) { return __uint_as_float((o >> 31) ? (o ^ 0x80000000u) : ~o); }
 __device__ __forceinline__ u64 rank_of(float v, int i) { return ((u64)(~mono(v)) << 32) | (unsigned)i; }
 __device__ __forceinline__ float rank_value(u64 c) { return unmono(~(unsigned)(c >> 32)); }
 
+// ---- reductions over a workgroup of NT threads (red: NT / 64 words of LDS; every call starts with a barrier) ---------------------
 __device__ __forceinline__ u64 shfl_xor_u64(u64 v, int o) {
     const unsigned lo = __shfl_xor((unsigned)v, o, 64), hi = __shfl_xor((unsigned)(v >> 32), o, 64);
     return ((u64)hi << 32) | lo;
@@ -49,7 +90,6 @@ __device__ __forceinline__ u64 shfl_up_u64(u64 v, int o) {
     const unsigned lo = __shfl_up((unsigned)v, o, 64), hi = __shfl_up((unsigned)(v >> 32), o, 64);
     return ((u64)hi << 32) | lo;
 }
-// smallest of all threads' values
 template <int NT> __device__ __forceinline__ u64 block_min(u64 v, u64* red) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) { const u64 x = shfl_xor_u64(v, o); v = x < v ? x : v; }
@@ -57,11 +97,23 @@ template <int NT> __device__ __forceinline__ u64 block_min(u64 v, u64* red) {
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     v = red[0];
+#pragma unroll
     for (int i = 1; i < NT / 64; ++i) v = red[i] < v ? red[i] : v;
     return v;
 }
-// exclusive prefix over the threads; *total = sum of all
-template <int NT> __device__ __forceinline__ u64 block_scan(u64 v, u64* red, u64* total) {
+template <int NT> __device__ __forceinline__ float block_max(float v, u64* red) {
+    v = wave_max(v);
+    float* r = (float*)red;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = r[0];
+#pragma unroll
+    for (int i = 1; i < NT / 64; ++i) v = fmaxf(v, r[i]);
+    return v;
+}
+// exclusive prefix over the threads; total = sum of all
+template <int NT> __device__ __forceinline__ u64 block_scan(u64 v, u64* red, u64& total) {
     u64 s = v;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) { const u64 x = shfl_up_u64(s, o); if ((int)(threadIdx.x & 63) >= o) s += x; }
@@ -69,47 +121,61 @@ template <int NT> __device__ __forceinline__ u64 block_scan(u64 v, u64* red, u64
     if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = s;
     __syncthreads();
     u64 before = 0, all = 0;
+#pragma unroll
     for (int i = 0; i < NT / 64; ++i) { if (i < (int)(threadIdx.x >> 6)) before += red[i]; all += red[i]; }
-    *total = all;
+    total = all;
     return before + s - v;
 }
 
-// z - z_max of a value, and its mass
-struct Weigh {
-    double top, inv_t; double scale;
-    __device__ __forceinline__ double x(float v) const { return v == -INFINITY ? -INFINITY : ((double)v - top) * inv_t; }
-    __device__ __forceinline__ u64 mass(double x) const { return x < -50.0 ? 0ull : (u64)__builtin_fma(exp(x), scale, 0.5); }   // (spelled out: the same bits at every place that weighs a token)
-};
-
-// the rank-th smallest entry of the list by COUNT (need = how many, >= 1), or the smallest entry at which the running MASS reaches
-// `need`; ~0 if the whole list does not.  Eight passes of eight bits from the top.
-template <int NT> __device__ u64 select_rank(const u64* list, int n, bool by_mass, u64 need, const Weigh& w, u64* hist /*[256]*/, u64* red) {
-    u64 prefix = 0, got = 0;
-    for (int shift = 56; shift >= 0; shift -= 8) {
-        __syncthreads();
-        if (threadIdx.x < 256) hist[threadIdx.x] = 0;
-        __syncthreads();
-        for (int i = threadIdx.x; i < n; i += NT) {
-            const u64 c = list[i];
-            if (shift < 56 && (c >> (shift + 8)) != (prefix >> (shift + 8))) continue;
-            const u64 a = by_mass ? w.mass(w.x(rank_value(c))) : 1ull;
-            atomicAdd(&hist[(c >> shift) & 255], a);
-        }
-        __syncthreads();
-        u64 total;
-        const u64 mine = threadIdx.x < 256 ? hist[threadIdx.x] : 0ull;
-        const u64 before = got + block_scan<NT>(mine, red, &total);
-        // the first digit whose running sum reaches `need`
-        const bool hit = threadIdx.x < 256 && before < need && before + mine >= need;
-        const u64 d = block_min<NT>(hit ? ((u64)threadIdx.x) : ~0ull, red);
-        if (d == ~0ull) return ~0ull;
-        const u64 b = block_min<NT>(threadIdx.x == d ? before : ~0ull, red);
-        prefix |= d << shift;
-        got = b;
-    }
-    return prefix;
+// ---- weights ------------------------------------------------------------------------------------------------------------------------
+// exp(-at / 64), at >= 0: exp(-floor(at) / 64) from two tables (of 32 and 64 entries), the rest from the series
+struct ExpTab { double a[32], b[64]; };
+__device__ __forceinline__ void exp_tab_init(ExpTab& t) {
+    if (threadIdx.x < 32) t.a[threadIdx.x] = exp(-(double)threadIdx.x);
+    else if (threadIdx.x >= 64 && threadIdx.x < 128) t.b[threadIdx.x - 64] = exp(-(double)(threadIdx.x - 64) / 64.0);
 }
-
+__device__ __forceinline__ double exp_tab(const ExpTab& t, int n) { return t.a[n >> 6] * t.b[n & 63]; }
+// exp(y) - 1, |y| <= 1/64 (y^7 / 5040 = 4e-17)
+__device__ __forceinline__ double expm1_64(double y) {
+    double p = 1.0 / 720.0;
+    p = __builtin_fma(p, y, 1.0 / 120.0); p = __builtin_fma(p, y, 1.0 / 24.0); p = __builtin_fma(p, y, 1.0 / 6.0);
+    p = __builtin_fma(p, y, 0.5); p = __builtin_fma(p, y, 1.0);
+    return p * y;
+}
+// x in [0, 2^51] rounded to a whole number: the low bits of 2^52 + x
+__device__ __forceinline__ u64 whole(double x) { return (u64)__double_as_longlong(x + 4503599627370496.0) - 0x4330000000000000ull; }
+struct Weigh {
+    const ExpTab* tab; double top, s, scale, amax;             // s = 64 / T; amax: min-p as a bound of at
+    __device__ __forceinline__ Weigh(const ExpTab* t, float top_, const Settings& st, int frac) {
+        tab = t; top = top_; s = 64.0 / (double)st.T; scale = (double)(1ull << frac);
+        amax = st.use_m ? -64.0 * log((double)fminf(st.M, 1.0f)) : INFINITY;
+    }
+    // 64 (z_max - z); SMP_BINS and more: no weight
+    __device__ __forceinline__ double at(float v) const { return v == -INFINITY ? 1e300 : (top - (double)v) * s; }
+    __device__ __forceinline__ u64 mass(double at) const {
+        if (!(at < (double)SMP_BINS)) return 0;
+        const int n = (int)at;
+        const double e = exp_tab(*tab, n);
+        return whole(__builtin_fma(e, expm1_64((at - (double)n) * (-1.0 / 64.0)), e) * scale);
+    }
+    // what counts in the draw
+    __device__ __forceinline__ u64 kept(float v, int i, u64 cut) const {
+        const double x = at(v);
+        return x <= amax && rank_of(v, i) <= cut ? mass(x) : 0;
+    }
+};
+// floor(u * all), exact; u outside [0, 1) is moved to its nearest end
+__device__ __forceinline__ u64 u_times(float u, u64 all) {
+    if (!(u > 0.0f)) u = 0.0f;
+    u = fminf(u, 0x1.fffffep-1f);
+    const u64 U = (u64)((double)u * 0x1p63);
+    return (__umul64hi(all, U) << 1) | ((all * U) >> 63);
+}
+// p of a mass, as the smallest whole number that a prefix has to reach (at least one token is kept)
+__device__ __forceinline__ u64 p_need(float P, u64 mass) {
+    const u64 n = (u64)ceil(P > 0.0f ? (double)P * (double)mass : 0.0);
+    return n < 1 ? 1 : n;
+}
 __device__ __forceinline__ void sample_store(const SampleArgs& a, int b, int token, float lp) {
     if (a.done) {
         const int dn = a.done[b], tk = token < 0 ? a.eos : token;      // a row with nothing to draw from ends its sentence
@@ -122,146 +188,522 @@ __device__ __forceinline__ void sample_store(const SampleArgs& a, int b, int tok
         if (a.logprob) a.logprob[b] = lp;
     }
 }
+__device__ __forceinline__ float log_prob(const Weigh& w, double at, u64 all) { return (float)(at * (-1.0 / 64.0) - log((double)all / w.scale)); }
 
-template <bool BF16> __global__ __launch_bounds__(SMP_NT) void k_sample_row(SampleArgs a) {
-    constexpr int NT = SMP_NT;
-    __shared__ u64 red[NT / 64];
-    __shared__ u64 mass[SMP_BINS];
-    __shared__ unsigned cnt[SMP_BINS];
-    __shared__ u64 hist[256];
-    __shared__ unsigned nlist;
-    __shared__ u64 zone_s[4];
-    const int b = blockIdx.x, tid = threadIdx.x, V = a.V;
-    const char* row = (const char*)a.logits + (size_t)b * a.ldl * (BF16 ? 2 : 4);
-    const float T = a.t ? a.t[b] : a.t0;
-    const float P = a.p ? a.p[b] : a.p0, Mp = a.m ? a.m[b] : a.m0;
-    const int k = a.k ? a.k[b] : a.k0;
-    const bool use_p = P < 1.0f, use_k = k > 0 && k < V, use_m = Mp > 0.0f;
-    u64 best = ~0ull;
-    for (int i = tid; i < V; i += NT) { const u64 c = rank_of(logit_at<BF16>(row, i), i); best = c < best ? c : best; }
-    best = block_min<NT>(best, red);
-    const float top = rank_value(best);
-    if (top == -INFINITY) { if (tid == 0) sample_store(a, b, -1, -INFINITY); return; }
-    if (!(T > 0.0f)) { if (tid == 0) sample_store(a, b, (int)(unsigned)best, 0.0f); return; }
-    Weigh w;
-    w.top = top; w.inv_t = 1.0 / (double)T; w.scale = (double)(1ull << a.frac);
-    const double xmin = use_m ? log((double)fminf(Mp, 1.0f)) : -INFINITY;
-    u64 cut = ~0ull;
-    if (use_k || use_p) {
-        for (int i = tid; i < SMP_BINS; i += NT) { mass[i] = 0; cnt[i] = 0; }
-        if (tid == 0) { nlist = 0; zone_s[0] = zone_s[1] = ~0ull; }
+// ---- ranking a few tokens among themselves -----------------------------------------------------------------------------------------
+// Of the tokens with rank <= hi that `each` enumerates (at most n, each by exactly one thread): the need-th by count (BY_MASS false; there are
+// as many), or the first at which the running mass reaches need -- the last one where the whole does not; `mass_to`: the mass up to
+// and with it.  While there are more than CAP: a histogram over the eight highest bits in which they differ.
+template <int NT> struct SelectLds {
+    static constexpr int CAP = NT >= 1024 ? 256 : NT >= 512 ? 180 : 128;       // (n^2 / NT steps to rank n)
+    u64 m[256]; unsigned c[256];
+    u64 list[CAP], lm[CAP];
+    unsigned n;
+    u64 out[3];
+};
+template <int NT, bool BY_MASS, class Each> __device__ __forceinline__ u64 select_rank(Each each, u64 hi, int n, u64 need, const Weigh& w, SelectLds<NT>& L, u64* red,
+                                                                                      u64& mass_to) {
+    u64 lo = 0, before_m = 0, before_c = 0;
+    while (n > SelectLds<NT>::CAP) {
+        u64 mn = ~0ull, mx = ~0ull;
+        each([&](u64 r) { if (r >= lo && r <= hi) { mn = r < mn ? r : mn; mx = ~r < mx ? ~r : mx; } });
+        mn = block_min<NT>(mn, red); mx = ~block_min<NT>(mx, red);
+        if (mn > mx) { mass_to = before_m; return ~0ull; }                 // (nothing there)
+        const int shift = max(0, 56 - (mn == mx ? 64 : (int)__clzll((long long)(mn ^ mx))));
+        for (int i = threadIdx.x; i < 256; i += NT) { L.m[i] = 0; L.c[i] = 0; }
         __syncthreads();
-        for (int i = tid; i < V; i += NT) {
-            const double x = w.x(logit_at<BF16>(row, i));
-            const double at = -x * SMP_PER_Z;
-            if (at < (double)SMP_BINS) { const int q = (int)at; atomicAdd(&cnt[q], 1u); atomicAdd(&mass[q], w.mass(x)); }
+        const u64 first = mn >> shift;
+        each([&](u64 r) {
+            if (r >= lo && r <= hi) { const int d = (int)((r >> shift) - first); atomicAdd(&L.c[d], 1u); atomicAdd(&L.m[d], w.mass(w.at(rank_value(r)))); }
+        });
+        __syncthreads();
+        const u64 mc = threadIdx.x < 256 ? L.c[threadIdx.x] : 0, mm = threadIdx.x < 256 ? L.m[threadIdx.x] : 0;
+        u64 tc, tm;
+        const u64 bc = before_c + block_scan<NT>(mc, red, tc), bm = before_m + block_scan<NT>(mm, red, tm);
+        const u64 b = BY_MASS ? bm : bc, x = BY_MASS ? mm : mc, most = BY_MASS ? before_m + tm : before_c + tc, nd = need < most ? need : most;
+        if (threadIdx.x < 256 && b < nd && b + x >= nd) { L.out[0] = threadIdx.x; L.out[1] = bc; L.out[2] = bm; }
+        __syncthreads();
+        const u64 d = L.out[0];
+        before_c = L.out[1]; before_m = L.out[2];
+        const u64 l2 = (first + d) << shift, h2 = l2 + ((1ull << shift) - 1);
+        lo = l2 > lo ? l2 : lo; hi = h2 < hi ? h2 : hi;
+        n = (int)L.c[d];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) L.n = 0;
+    __syncthreads();
+    each([&](u64 r) { if (r >= lo && r <= hi) { const unsigned k = atomicAdd(&L.n, 1u); if (k < (unsigned)SelectLds<NT>::CAP) { L.list[k] = r; L.lm[k] = w.mass(w.at(rank_value(r))); } } });
+    __syncthreads();
+    n = (int)L.n;
+    if (n == 0) { mass_to = before_m; return ~0ull; }
+    // g threads (a power of two, within a wave) share the comparisons of one token
+    int g = 1;
+    while (g < 64 && n * g * 2 <= NT) g *= 2;
+    const int e = threadIdx.x / g, part = threadIdx.x & (g - 1);
+    u64 c = 0, m = 0, mine = 0, own = 0;
+    if (e < n) {
+        mine = L.list[e]; own = L.lm[e];
+        for (int i = part; i < n; i += g) if (L.list[i] <= mine) { ++c; m += L.lm[i]; }
+    }
+    for (int o = 1; o < g; o <<= 1) { c += shfl_xor_u64(c, o); m += shfl_xor_u64(m, o); }
+    if (e < n && part == 0 && c == (u64)n) L.out[2] = m;     // (the last of them: the mass of all)
+    __syncthreads();
+    const u64 most = before_m + L.out[2];
+    if (e < n && part == 0) {
+        const u64 nd = BY_MASS ? (need < most ? need : most) : need;
+        const u64 x = BY_MASS ? before_m + m : before_c + c, b = BY_MASS ? x - own : x - 1;
+        if (b < nd && x >= nd) { L.out[0] = mine; L.out[1] = before_m + m; }
+    }
+    __syncthreads();
+    const u64 r = L.out[0];
+    mass_to = L.out[1];
+    __syncthreads();
+    return r;
+}
+
+// ---- one workgroup a row ---------------------------------------------------------------------------------------------------------------
+template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sample_row(SampleArgs a) {
+    constexpr int E = Row<BF16>::E, NG = VPT / E, PER = SMP_BINS / NT;
+    __shared__ u64 red[NT / 64];
+    __shared__ ExpTab tab;
+    __shared__ u64 hist[SMP_BINS];
+    __shared__ SelectLds<NT> L;
+    __shared__ u64 zs[4];
+    const int b = blockIdx.x, tid = threadIdx.x;
+    const Row<BF16> row(a, b);
+    const Settings st = settings_of(a, b);
+    const float u = a.u[b];
+    // thread t holds tokens t * VPT - o .. + VPT - 1
+    float v[VPT];
+#pragma unroll
+    for (int q = 0; q < NG; ++q) row.group(tid * NG + q, v + q * E);
+    const int i0 = tid * VPT - row.o;
+    exp_tab_init(tab);
+    float top = v[0];
+#pragma unroll
+    for (int j = 1; j < VPT; ++j) top = fmaxf(top, v[j]);
+    top = block_max<NT>(top, red);
+    if (top == -INFINITY) { if (tid == 0) sample_store(a, b, -1, -INFINITY); return; }
+    if (st.greedy) {
+        u64 best = ~0ull;
+#pragma unroll
+        for (int j = VPT - 1; j >= 0; --j) if (v[j] == top) best = (u64)(unsigned)(i0 + j);
+        best = block_min<NT>(best, red);
+        if (tid == 0) sample_store(a, b, (int)best, 0.0f);
+        return;
+    }
+    const Weigh w(&tab, top, st, a.frac);
+    u64 cut = ~0ull;
+    if (st.use_k || st.use_p) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) hist[tid * PER + j] = 0;
+        if (tid == 0) zs[0] = zs[1] = ~0ull;
+        __syncthreads();
+        // one word a token: 1 << 48 for the count, and 2^39 (1 - exp(-rest / 64)) of what the bin's edge exceeds it by (below 16384 / 64)
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const double at = w.at(v[j]);
+            if (at < (double)SMP_BINS) {
+                const int n = (int)at;
+                atomicAdd(&hist[n], (1ull << 48) + whole(-expm1_64((at - (double)n) * (-1.0 / 64.0)) * 0x1p39));
+            }
         }
         __syncthreads();
-        constexpr int PER = SMP_BINS / NT;
         u64 c[PER], m[PER], cs = 0, ms = 0;
-        for (int j = 0; j < PER; ++j) { c[j] = cnt[tid * PER + j]; m[j] = mass[tid * PER + j]; cs += c[j]; ms += m[j]; }
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const u64 h = hist[tid * PER + j];
+            c[j] = h >> 48;
+            m[j] = (u64)(((double)c[j] - (double)(long long)(h & 0xFFFFFFFFFFFFull) * 0x1p-39) * exp_tab(tab, tid * PER + j) * w.scale + 0.5);
+            cs += c[j]; ms += m[j];
+        }
         u64 call, mall;
-        const u64 cb = block_scan<NT>(cs, red, &call), mb = block_scan<NT>(ms, red, &mall);
-        // the bin that holds the k-th token, the mass in front of it and with it
+        const u64 cb = block_scan<NT>(cs, red, call), mb = block_scan<NT>(ms, red, mall);
+        // tokens of one bin, by rank
+        auto in_bin = [&](int bin) {
+            return [&, bin](auto f) {
+#pragma unroll
+                for (int j = 0; j < VPT; ++j) {
+                    const double at = w.at(v[j]);
+                    if (at < (double)SMP_BINS && (int)at == bin) f(rank_of(v[j], i0 + j));
+                }
+            };
+        };
+        u64 mass = mall;
         int bk = SMP_BINS;
-        u64 zlo = mall, zhi = mall;
-        const bool cut_k = use_k && (u64)k < call;
-        if (cut_k) {
+        if (st.use_k && (u64)st.k < call) {
             u64 cc = cb, mm = mb;
+#pragma unroll
             for (int j = 0; j < PER; ++j) {
-                if (cc < (u64)k && cc + c[j] >= (u64)k) { zone_s[0] = (u64)(tid * PER + j); zone_s[2] = mm; zone_s[3] = mm + m[j]; }
+                if (cc < (u64)st.k && cc + c[j] >= (u64)st.k) { zs[0] = (u64)(tid * PER + j); zs[2] = cc | (c[j] << 32); zs[3] = mm; }
                 cc += c[j]; mm += m[j];
             }
             __syncthreads();
-            bk = (int)zone_s[0]; zlo = zone_s[2]; zhi = zone_s[3];
+            bk = (int)zs[0];
+            const u64 before = zs[2] & 0xFFFFFFFFull, above = zs[3];
+            u64 to;
+            cut = select_rank<NT, false>(in_bin(bk), ~0ull, (int)(zs[2] >> 32), (u64)st.k - before, w, L, red, to);
+            mass = above + to;
         }
-        // the first bin in which the running mass can reach p of the whole (whose mass is zlo .. zhi until the k-th token is known)
-        int b0 = bk;
-        if (use_p) {
-            const double need = P > 0.0f ? (double)P * (double)zlo : 0.0;
-            u64 nd = (u64)ceil(need); if (nd < 1) nd = 1;
+        if (st.use_p) {
+            const u64 need = p_need(st.P, mass);
             u64 mm = mb;
-            for (int j = 0; j < PER; ++j) { if (mm < nd && mm + m[j] >= nd) zone_s[1] = (u64)(tid * PER + j); mm += m[j]; }
             __syncthreads();
-            if (zone_s[1] != ~0ull) b0 = min(bk, (int)zone_s[1]);
-        }
-        int b1 = cut_k ? bk : b0;
-        __syncthreads();
-        if (b0 < SMP_BINS) {
-            // count and mass in front of the zone
-            if (tid * PER <= b0 && b0 < (tid + 1) * PER) {
-                u64 cc = cb, mm = mb;
-                for (int j = 0; tid * PER + j < b0; ++j) { cc += c[j]; mm += m[j]; }
-                zone_s[2] = cc; zone_s[3] = mm;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                if (tid * PER + j <= bk && mm < need && mm + m[j] >= need) { zs[1] = (u64)(tid * PER + j); zs[2] = c[j]; zs[3] = mm; }
+                mm += m[j];
             }
-            u64* list = a.list + (size_t)b * V;
-            for (int i = tid; i < V; i += NT) {
-                const float v = logit_at<BF16>(row, i);
-                const double at = -w.x(v) * SMP_PER_Z;
-                if (at < (double)(b1 + 1) && at >= (double)b0) list[atomicAdd(&nlist, 1u)] = rank_of(v, i);
-            }
-            __threadfence_block();
             __syncthreads();
-            const int n = (int)nlist;
-            const u64 nabove = zone_s[2], above = zone_s[3];
-            u64 whole = mall;
-            if (cut_k) {
-                cut = select_rank<NT>(list, n, false, (u64)k - nabove, w, hist, red);
-                u64 s = 0;
-                for (int i = tid; i < n; i += NT) if (list[i] <= cut) s += w.mass(w.x(rank_value(list[i])));
-                block_scan<NT>(s, red, &whole);
-                whole += above;
-            }
-            if (use_p) {
-                u64 nd = (u64)ceil(P > 0.0f ? (double)P * (double)whole : 0.0); if (nd < 1) nd = 1;
-                if (nd > above) { const u64 cp = select_rank<NT>(list, n, true, nd - above, w, hist, red); cut = cp < cut ? cp : cut; }
+            if (zs[1] != ~0ull) {
+                u64 to;
+                const u64 cp = select_rank<NT, true>(in_bin((int)zs[1]), cut, (int)zs[2], need - zs[3], w, L, red, to);
+                cut = cp < cut ? cp : cut;
             }
         }
     }
     // the draw: running sums in the order of the vocabulary
-    const int per = (V + NT - 1) / NT;
-    const int i0 = min(V, tid * per), i1 = min(V, i0 + per);
     u64 s = 0;
-    for (int i = i0; i < i1; ++i) {
-        const float v = logit_at<BF16>(row, i);
-        const double x = w.x(v);
-        if (x >= xmin && rank_of(v, i) <= cut) s += w.mass(x);
-    }
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) s += w.kept(v[j], i0 + j, cut);
     u64 all;
-    u64 before = block_scan<NT>(s, red, &all);
-    float u = a.u[b];
-    if (!(u > 0.0f)) u = 0.0f;
-    u = fminf(u, 0x1.fffffep-1f);
-    const u64 U = (u64)((double)u * 0x1p63);
-    const u64 r = (__umul64hi(all, U) << 1) | ((all * U) >> 63);          // floor(u * all), exact
+    u64 before = block_scan<NT>(s, red, all);
+    const u64 r = u_times(u, all);
     if (before <= r && r < before + s) {
-        for (int i = i0; i < i1; ++i) {
-            const float v = logit_at<BF16>(row, i);
-            const double x = w.x(v);
-            if (x >= xmin && rank_of(v, i) <= cut) {
-                const u64 m = w.mass(x);
-                if (r < before + m) { sample_store(a, b, i, (float)(x - log((double)all / w.scale))); break; }
-                before += m;
-            }
+        int pick = -1; float pv = 0.f;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const u64 m = w.kept(v[j], i0 + j, cut);
+            if (pick < 0 && r < before + m) { pick = i0 + j; pv = v[j]; }
+            before += m;
         }
+        sample_store(a, b, pick, log_prob(w, w.at(pv), all));
     }
 }
 
+// ---- long rows ----------------------------------------------------------------------------------------------------------------------
+// Four launches: k_sample_hist (the row's only whole pass: chunks' histograms, tile maxima), k_sample_zone (which bins hold the cut),
+// k_sample_gather (mass above the cut of every tile that reaches it, and a list of the tokens in the cut's bins), k_sample_draw (the cut, the
+// tile, the token).  Tiles whose maximum lies below the cut are not read again.
+//
+// A chunk counts before the row's maximum is known (a pass over the logits less): its bins are whole parts of (l - ref) 64 / T from a
+// reference of its own, so they lie across the row's bins floor(64 (z_max - z)).  A token of chunk bin y -- in the row's units -- belongs to
+// the row's bin y - 1 or y; entered at y - 1 throughout, the running sums bound the true ones from above, and one bin on from below:
+// the cut's bin is one of two.  The masses themselves are exact to 1e-13: bin edge times (count + what the tokens exceed it by).
+struct ZoneRec {
+    u64 best;                 // rank of the row's first token (~0: none)
+    u64 whole;                // mass of all tokens
+    int b0, b1;               // bins whose tokens are ranked one by one; in front of b0 everything is kept, behind b1 nothing
+    int cut_k, cut_p;         // what is to be found in them
+    unsigned n;               // tokens in them
+};
+struct Chunk { double ref, g_top; u64 best; };                 // bin 0 holds tokens with floor((l - ref) 64 / T) = g_top
+struct Tile { u64 all, kept; float top; unsigned count; };     // in front of b0: mass, mass that min-p leaves, tokens; the tile's largest logit
+struct RowWs { u64* hist; Chunk* chunk; Tile* tile; ZoneRec* rec; u64* list; };
+static inline __host__ __device__ size_t ws_up(size_t n) { return (n + 15) & ~(size_t)15; }
+static inline __host__ __device__ size_t row_ws_bytes(int G, int tiles) {
+    return (size_t)G * SMP_BINS * 8 + ws_up(G * sizeof(Chunk)) + ws_up(tiles * sizeof(Tile)) + ws_up(sizeof(ZoneRec)) + (size_t)SMP_LIST * 8;
+}
+__device__ __forceinline__ RowWs row_ws(const SampleArgs& a, int b) {
+    RowWs r;
+    char* p = a.ws + (size_t)b * row_ws_bytes(a.G, a.tiles);
+    r.hist = (u64*)p; p += (size_t)a.G * SMP_BINS * 8;
+    r.chunk = (Chunk*)p; p += ws_up(a.G * sizeof(Chunk));
+    r.tile = (Tile*)p; p += ws_up(a.tiles * sizeof(Tile));
+    r.rec = (ZoneRec*)p; p += ws_up(sizeof(ZoneRec));
+    r.list = (u64*)p;
+    return r;
+}
+template <bool BF16> __global__ __launch_bounds__(256) void k_sample_hist(SampleArgs a) {
+    constexpr int NT = 256, E = Row<BF16>::E, TG = SMP_TILE / E, NQ = TG / NT;
+    __shared__ u64 red[NT / 64];
+    __shared__ u64 ring[SMP_BINS];
+    const int chunk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+    const Row<BF16> row(a, b);
+    const Settings st = settings_of(a, b);
+    const bool bins = !st.greedy && (st.use_k || st.use_p);
+    const RowWs ws = row_ws(a, b);
+    const int t0 = (int)((long long)chunk * a.tiles / a.G), t1 = (int)((long long)(chunk + 1) * a.tiles / a.G);
+    const double sc = 64.0 / (double)st.T;
+    double ref = 0.0, g_top = -INFINITY;                   // bin 0 of the ring, at place `head`; lower bins lie in front of it
+    int head = 0;
+    float bv = -INFINITY; int bi = 0;
+    for (int t = t0; t < t1; ++t) {
+        float v[NQ * E];
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) row.group(t * TG + q * NT + tid, v + q * E);
+        float mx = -INFINITY;
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float x = v[q * E + e];
+                mx = fmaxf(mx, x);
+                if (x > bv) { bv = x; bi = (t * TG + q * NT + tid) * E - row.o + e; }       // (a thread's places ascend: the first of equals stays)
+            }
+        mx = block_max<NT>(mx, red);
+        if (tid == 0) ws.tile[t].top = mx;
+        if (!bins || mx == -INFINITY) continue;
+        const double g = floor(((double)mx - ref) * sc);
+        if (!(g - g_top < (double)SMP_BINS)) {             // the first tokens, or all before lie below the window: start anew from here
+            ref = (double)mx; g_top = 0.0; head = 0;
+            for (int i = tid; i < SMP_BINS; i += NT) ring[i] = 0;
+            __syncthreads();
+        } else if (g > g_top) {                            // the window moves up: its new bins start empty
+            const int nz = (int)(g - g_top);
+            for (int i = tid; i < nz; i += NT) ring[(head + 1 + i) & (SMP_BINS - 1)] = 0;
+            head = (head + nz) & (SMP_BINS - 1);
+            g_top = g;
+            __syncthreads();
+        }
+        // one word a token: 1 << 48 for the count, and 2^38 (exp(rest / 64) - 1) of what it exceeds the bin's edge by (49152 tokens: below 2^48)
+#pragma unroll
+        for (int j = 0; j < NQ * E; ++j) {
+            const double x = ((double)v[j] - ref) * sc, fl = floor(x), rel = g_top - fl;
+            if (rel < (double)SMP_BINS) atomicAdd(&ring[(head - (int)rel) & (SMP_BINS - 1)], (1ull << 48) + whole(expm1_64((x - fl) * (1.0 / 64.0)) * 0x1p38));
+        }
+    }
+    const u64 best = block_min<NT>(bv == -INFINITY ? ~0ull : rank_of(bv, bi), red);
+    if (tid == 0) { ws.chunk[chunk].best = best; ws.chunk[chunk].ref = ref; ws.chunk[chunk].g_top = g_top; }
+    if (bins && best != ~0ull) for (int i = tid; i < SMP_BINS; i += NT) ws.hist[(size_t)chunk * SMP_BINS + i] = ring[(head - i) & (SMP_BINS - 1)];
+}
+
+#define SMP_TILES_MAX (E2T_SAMPLE_MAX_V / SMP_TILE + 1)
+__global__ __launch_bounds__(1024) void k_sample_zone(SampleArgs a) {
+    constexpr int NT = 1024, PER = SMP_BINS / NT;
+    __shared__ u64 red[NT / 64];
+    __shared__ ExpTab tab;
+    __shared__ u64 zs[4];
+    __shared__ double edge[SMP_TILES_MAX];
+    __shared__ int shift[SMP_TILES_MAX];
+    const int b = blockIdx.x, tid = threadIdx.x;
+    const Settings st = settings_of(a, b);
+    const RowWs ws = row_ws(a, b);
+    ZoneRec& rec = *ws.rec;
+    exp_tab_init(tab);
+    u64 best = tid < a.G ? ws.chunk[tid].best : ~0ull;
+    best = block_min<NT>(best, red);
+    if (tid == 0) { rec.best = best; rec.n = 0; rec.whole = 0; rec.cut_k = rec.cut_p = 0; rec.b0 = SMP_BINS + 1; rec.b1 = SMP_BINS; }
+    if (best == ~0ull || st.greedy || (!st.use_k && !st.use_p)) return;
+    if (tid < a.G) {
+        const Chunk c = ws.chunk[tid];
+        // the chunk's bin 0 lies at d .. of the row's units (>= 0: the row's largest is no smaller than the chunk's)
+        const double d = c.best == ~0ull ? 1e300 : fmax(((double)rank_value(best) - c.ref) * (64.0 / (double)st.T) - c.g_top, 0.0), fl = floor(d);
+        shift[tid] = fl < (double)SMP_BINS ? (int)fl : SMP_BINS;
+        edge[tid] = fl < (double)SMP_BINS ? exp((d - fl) * (-1.0 / 64.0)) * (double)(1ull << a.frac) : 0.0;
+    }
+    if (tid == 0) zs[0] = zs[1] = ~0ull;
+    __syncthreads();
+    u64 c[PER], m[PER], cs = 0, ms = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int x = tid * PER + j;
+        u64 cn = 0, mass = 0;
+        for (int k = 0; k < a.G; ++k) {
+            const u64* h = ws.hist + (size_t)k * SMP_BINS;
+            const int r = x + 1 - shift[k];                // the chunk's bin that covers the row's bins x and x + 1
+            if (r >= 0 && r < SMP_BINS && x + 1 < SMP_BINS) {
+                const u64 w = h[r];
+                cn += w >> 48; mass += (u64)(((double)(w >> 48) + (double)(w & 0xFFFFFFFFFFFFull) * 0x1p-38) * exp_tab(tab, x + 1) * edge[k] + 0.5);
+            }
+            if (x == 0 && shift[k] == 0) {
+                const u64 w = h[0];
+                cn += w >> 48; mass += (u64)(((double)(w >> 48) + (double)(w & 0xFFFFFFFFFFFFull) * 0x1p-38) * edge[k] + 0.5);
+            }
+        }
+        c[j] = cn; m[j] = mass; cs += cn; ms += mass;
+    }
+    u64 call, mall;
+    const u64 cb = block_scan<NT>(cs, red, call), mb = block_scan<NT>(ms, red, mall);
+    int bk = SMP_BINS;
+    u64 least = mall;                                      // the top-k's mass is at least this
+    const bool cut_k = st.use_k && (u64)st.k < call;
+    if (cut_k) {
+        u64 cc = cb;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) { if (cc < (u64)st.k && cc + c[j] >= (u64)st.k) zs[0] = (u64)(tid * PER + j); cc += c[j]; }
+        __syncthreads();
+        bk = (int)zs[0];
+        // bins in front of bk lie in the top-k; their mass is at least what is entered in front of bk - 1
+        if (bk - 1 >= tid * PER && bk - 1 < (tid + 1) * PER) { u64 mm = mb; for (int j = 0; tid * PER + j < bk - 1; ++j) mm += m[j]; zs[2] = mm; }
+        __syncthreads();
+        least = bk >= 1 ? zs[2] : 0;
+    }
+    int b0 = bk;
+    if (st.use_p) {
+        const u64 need = p_need(st.P, least);
+        u64 mm = mb;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) { if (mm < need && mm + m[j] >= need) zs[1] = (u64)(tid * PER + j); mm += m[j]; }
+        __syncthreads();
+        if (zs[1] != ~0ull) b0 = min(bk, (int)zs[1]);
+    }
+    if (tid == 0 && b0 < SMP_BINS) { rec.whole = mall; rec.b0 = b0; rec.b1 = (cut_k ? bk : b0) + 1; rec.cut_k = cut_k; rec.cut_p = st.use_p; }
+}
+
+template <bool BF16> __global__ __launch_bounds__(256) void k_sample_gather(SampleArgs a) {
+    constexpr int NT = 256, E = Row<BF16>::E, TG = SMP_TILE / E, NQ = TG / NT;
+    __shared__ u64 red[NT / 64];
+    __shared__ ExpTab tab;
+    const int t = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+    const Settings st = settings_of(a, b);
+    const RowWs ws = row_ws(a, b);
+    ZoneRec& rec = *ws.rec;
+    if (st.greedy || rec.best == ~0ull) return;
+    const Row<BF16> row(a, b);
+    const Weigh w(&tab, rank_value(rec.best), st, a.frac);
+    const double b0 = rec.b0, b1 = rec.b1;
+    const float mx = ws.tile[t].top;
+    if (!(floor(w.at(mx)) <= b1)) { if (tid == 0) { ws.tile[t].all = ws.tile[t].kept = 0; ws.tile[t].count = 0; } return; }
+    exp_tab_init(tab);
+    float v[NQ * E];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) row.group(t * TG + q * NT + tid, v + q * E);
+    __syncthreads();
+    u64 s = 0, sk = 0;
+    unsigned cnt = 0;
+#pragma unroll
+    for (int j = 0; j < NQ * E; ++j) {
+        const double x = w.at(v[j]), bin = floor(x);
+        if (bin < b0 && x < (double)SMP_BINS) { const u64 m = w.mass(x); s += m; ++cnt; if (x <= w.amax) sk += m; }
+        const bool in = bin >= b0 && bin <= b1;
+        const u64 vote = __ballot(in);
+        if (vote) {
+            unsigned base = 0;
+            const int lane = tid & 63, first = __ffsll((long long)vote) - 1;
+            if (lane == first) base = atomicAdd(&rec.n, (unsigned)__popcll(vote));
+            base = __shfl(base, first, 64);
+            if (in) {
+                const unsigned k = base + (unsigned)__popcll(vote & ((1ull << lane) - 1));
+                if (k < SMP_LIST) ws.list[k] = rank_of(v[j], (t * TG + (j / E) * NT + tid) * E - row.o + j % E);
+            }
+        }
+    }
+    u64 all, kept, count;
+    block_scan<NT>(s, red, all);
+    block_scan<NT>(sk, red, kept);
+    block_scan<NT>((u64)cnt, red, count);
+    if (tid == 0) { ws.tile[t].all = all; ws.tile[t].kept = kept; ws.tile[t].count = (unsigned)count; }
+}
+
+template <bool BF16> __global__ __launch_bounds__(1024) void k_sample_draw(SampleArgs a) {
+    constexpr int NT = 1024, E = Row<BF16>::E, TG = SMP_TILE / E;
+    __shared__ u64 red[NT / 64];
+    __shared__ ExpTab tab;
+    __shared__ SelectLds<NT> L;
+    __shared__ u64 tsum[SMP_TILES_MAX];
+    __shared__ u64 zs[2];
+    const int b = blockIdx.x, tid = threadIdx.x;
+    const Settings st = settings_of(a, b);
+    const RowWs ws = row_ws(a, b);
+    const ZoneRec rec = *ws.rec;
+    if (rec.best == ~0ull) { if (tid == 0) sample_store(a, b, -1, -INFINITY); return; }
+    if (st.greedy) { if (tid == 0) sample_store(a, b, (int)(unsigned)rec.best, 0.0f); return; }
+    const Row<BF16> row(a, b);
+    exp_tab_init(tab);
+    const Weigh w(&tab, rank_value(rec.best), st, a.frac);
+    if (tid < a.tiles) tsum[tid] = ws.tile[tid].kept;
+    __syncthreads();
+    u64 cut = ~0ull;
+    if (rec.cut_k || rec.cut_p) {
+        u64 above, above_c;
+        block_scan<NT>(tid < a.tiles ? ws.tile[tid].all : 0, red, above);
+        block_scan<NT>(tid < a.tiles ? (u64)ws.tile[tid].count : 0, red, above_c);
+        // the tokens of the cut's bins: from the list, or, where they are more than it holds (a flat row), from the row itself
+        auto each = [&](auto f) {
+            if (rec.n <= SMP_LIST) { for (unsigned i = tid; i < rec.n; i += NT) f(ws.list[i]); }
+            else {
+                for (int q = tid; q < a.tiles * TG; q += NT) {
+                    float v[E];
+                    row.group(q, v);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const double bin = floor(w.at(v[e]));
+                        if (bin >= (double)rec.b0 && bin <= (double)rec.b1) f(rank_of(v[e], q * E - row.o + e));
+                    }
+                }
+            }
+        };
+        u64 to, mass = rec.whole;
+        if (rec.cut_k) { cut = select_rank<NT, false>(each, ~0ull, (int)rec.n, (u64)st.k - above_c, w, L, red, to); mass = above + to; }
+        if (rec.cut_p) {
+            const u64 need = p_need(st.P, mass);
+            const u64 cp = select_rank<NT, true>(each, cut, (int)rec.n, need > above ? need - above : 1, w, L, red, to);
+            cut = cp < cut ? cp : cut;
+        }
+        each([&](u64 r) {
+            if (r <= cut) {
+                const double x = w.at(rank_value(r));
+                if (x <= w.amax) atomicAdd(&tsum[((int)(unsigned)r + row.o) / SMP_TILE], w.mass(x));
+            }
+        });
+        __syncthreads();
+    }
+    const u64 s = tid < a.tiles ? tsum[tid] : 0;
+    u64 all;
+    const u64 before = block_scan<NT>(s, red, all);
+    const u64 r = u_times(a.u[b], all);
+    if (before <= r && r < before + s) { zs[0] = (u64)tid; zs[1] = before; }
+    __syncthreads();
+    const int t = (int)zs[0];
+    const u64 in_front = zs[1];
+    // the tile's tokens, in order: 4 (8) a thread
+    float v[E];
+    u64 ms = 0;
+    const int q = t * TG + tid, i0 = q * E - row.o;
+    if (tid < TG) {
+        row.group(q, v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) ms += w.kept(v[e], i0 + e, cut);
+    }
+    u64 x;
+    u64 at = in_front + block_scan<NT>(ms, red, x);
+    if (tid < TG && at <= r && r < at + ms) {
+        int pick = -1; float pv = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const u64 m = w.kept(v[e], i0 + e, cut);
+            if (pick < 0 && r < at + m) { pick = i0 + e; pv = v[e]; }
+            at += m;
+        }
+        sample_store(a, b, pick, log_prob(w, w.at(pv), all));
+    }
+}
+
+// ---- entry points -----------------------------------------------------------------------------------------------------------------------
+#define SMP_ROW_MAX (16384 - 7)         // (a row may start up to seven elements behind a 16-byte boundary)
 static int frac_bits(int V) { int c = 0; while ((1ll << c) < V) ++c; return 62 - c < 50 ? 62 - c : 50; }
-
-extern "C" size_t e2t_sample_ws_bytes(int B, int V) { return B > 0 && V > 0 ? (size_t)B * (size_t)V * sizeof(u64) : 0; }
-
+static int long_tiles(int V) { return (V + 7 + SMP_TILE - 1) / SMP_TILE; }
+// chunks of a long row: enough workgroups for the chip (1024 in all, a tile each at least), at most SMP_CHUNK_TILES tiles in one
+static int long_chunks(int B, int V) {
+    const int tiles = long_tiles(V), least = (tiles + SMP_CHUNK_TILES - 1) / SMP_CHUNK_TILES, want = (1024 + B - 1) / B;
+    return want < least ? least : want > tiles ? tiles : want;
+}
+extern "C" size_t e2t_sample_ws_bytes(int B, int V) {
+    return B > 0 && V > SMP_ROW_MAX && V <= E2T_SAMPLE_MAX_V ? (size_t)B * row_ws_bytes(long_chunks(B, V), long_tiles(V)) : 0;
+}
+template <bool BF16> static void sample_go(SampleArgs& a, int B, void* stream) {
+    if (a.V <= 2048 - 7) hipLaunchKernelGGL((k_sample_row<BF16, 256, 8>), dim3(B), dim3(256), 0, ST, a);
+    else if (a.V <= 8192 - 7) hipLaunchKernelGGL((k_sample_row<BF16, 512, 16>), dim3(B), dim3(512), 0, ST, a);
+    else if (a.V <= SMP_ROW_MAX) hipLaunchKernelGGL((k_sample_row<BF16, 1024, 16>), dim3(B), dim3(1024), 0, ST, a);
+    else {
+        hipLaunchKernelGGL((k_sample_hist<BF16>), dim3(a.G, B), dim3(256), 0, ST, a);
+        hipLaunchKernelGGL(k_sample_zone, dim3(B), dim3(1024), 0, ST, a);
+        hipLaunchKernelGGL((k_sample_gather<BF16>), dim3(a.tiles, B), dim3(256), 0, ST, a);
+        hipLaunchKernelGGL((k_sample_draw<BF16>), dim3(B), dim3(1024), 0, ST, a);
+    }
+}
 static int sample_launch(SampleArgs& a, int dtype, int B, const e2t_sample_cfg* cfg, void* ws, size_t ws_bytes, void* stream) {
-    E2T_CHECK_ARG(a.logits && a.u && cfg && B > 0 && a.V > 0 && a.V <= E2T_SAMPLE_MAX_V && a.ldl >= a.V);
+    E2T_CHECK_ARG(a.logits && a.u && cfg && B > 0 && B <= 65535 && a.V > 0 && a.V <= E2T_SAMPLE_MAX_V && a.ldl >= a.V);
     E2T_CHECK_ARG(dtype == E2T_DT_F32 || dtype == E2T_DT_BF16);
     E2T_CHECK_ARG(((uintptr_t)a.logits & (dtype == E2T_DT_F32 ? 3 : 1)) == 0);
-    E2T_CHECK_ARG(ws_bytes >= e2t_sample_ws_bytes(B, a.V) && (ws || !e2t_sample_ws_bytes(B, a.V)) && ((uintptr_t)ws & 15) == 0);
+    const size_t need = e2t_sample_ws_bytes(B, a.V);
+    E2T_CHECK_ARG(ws_bytes >= need && (ws || !need) && ((uintptr_t)ws & 15) == 0);
     a.frac = frac_bits(a.V);
     a.t0 = cfg->temperature; a.k0 = cfg->top_k; a.p0 = cfg->top_p; a.m0 = cfg->min_p;
     a.t = cfg->temperature_rows; a.k = cfg->top_k_rows; a.p = cfg->top_p_rows; a.m = cfg->min_p_rows;
-    a.list = (u64*)ws;
-    if (dtype == E2T_DT_BF16) hipLaunchKernelGGL((k_sample_row<true>), dim3(B), dim3(SMP_NT), 0, ST, a);
-    else hipLaunchKernelGGL((k_sample_row<false>), dim3(B), dim3(SMP_NT), 0, ST, a);
+    a.ws = (char*)ws; a.G = long_chunks(B, a.V); a.tiles = long_tiles(a.V);
+    if (dtype == E2T_DT_BF16) sample_go<true>(a, B, stream); else sample_go<false>(a, B, stream);
     E2T_LAUNCH_CHECK(); return E2T_OK;
 }
 extern "C" int e2t_sample_rows(const void* logits, int dtype, long long ldl, int B, int V, const float* u, const e2t_sample_cfg* cfg,
