@@ -36,7 +36,7 @@ struct SampleArgs {
     int* token; float* logprob;
     // bookkeeping of a decoder step (done == NULL: none)
     int l, Lmax, eos, pad; int *done, *out, *next_tok; float* score;
-    char* ws; int G, tiles;                                    // long rows: workspace, workgroups (chunks) and tiles a row
+    char* ws; int G, tiles;                                    // long rows: workspace, chunks and tiles of a row
 };
 struct Settings { float T, P, M; int k; bool use_k, use_p, use_m, greedy; };
 __device__ __forceinline__ Settings settings_of(const SampleArgs& a, int b) {
@@ -59,20 +59,35 @@ template <bool BF16> struct Row {
         o = (int)(((uintptr_t)row & 15) / (BF16 ? 2 : 4));
     }
     __device__ __forceinline__ float at(int i) const { return clean(BF16 ? bf2f(((const bf16_t*)row)[i]) : ((const float*)row)[i]); }
-    // E elements of group q; -inf outside the row
-    __device__ __forceinline__ void group(int q, float* v) const {
-        const int i = q * E - o;
-        if (i >= 0 && i + E <= V) {
-            const uint4 w = *(const uint4*)(row + (long long)i * (BF16 ? 2 : 4));
-            const unsigned x[4] = {w.x, w.y, w.z, w.w};
+    // n groups q0, q0 + step, ... as they lie (-inf outside the row); all loads leave before the first is looked at
+    template <int N> __device__ __forceinline__ void load(int q0, int step, uint4 (&w)[N]) const {
+        const int first = q0 * E - o, last = (q0 + (N - 1) * step) * E - o;
+        if (__all(first >= 0 && last + E <= V)) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) w[n] = *(const uint4*)(row + (long long)(first + n * step * E) * (BF16 ? 2 : 4));
+            return;
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int i = first + n * step * E;
+            unsigned x[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                if (BF16) { v[2 * e] = clean(__uint_as_float(x[e] << 16)); v[2 * e + 1] = clean(__uint_as_float(x[e] & 0xFFFF0000u)); }
-                else v[e] = clean(__uint_as_float(x[e]));
+                if (BF16) {
+                    const int k = i + 2 * e;
+                    const unsigned lo = k >= 0 && k < V ? ((const bf16_t*)row)[k] : 0xFF80u, hi = k + 1 >= 0 && k + 1 < V ? ((const bf16_t*)row)[k + 1] : 0xFF80u;
+                    x[e] = lo | (hi << 16);
+                } else x[e] = i + e >= 0 && i + e < V ? ((const unsigned*)row)[i + e] : 0xFF800000u;
             }
-        } else {
+            w[n] = make_uint4(x[0], x[1], x[2], x[3]);
+        }
+    }
+    static __device__ __forceinline__ void unpack(const uint4& w, float* v) {
+        const unsigned x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = i + e >= 0 && i + e < V ? at(i + e) : -INFINITY;
+        for (int e = 0; e < 4; ++e) {
+            if (BF16) { v[2 * e] = clean(__uint_as_float(x[e] << 16)); v[2 * e + 1] = clean(__uint_as_float(x[e] & 0xFFFF0000u)); }
+            else v[e] = clean(__uint_as_float(x[e]));
         }
     }
 };
@@ -82,30 +97,51 @@ __device__ __forceinline__ u64 rank_of(float v, int i) { return ((u64)(~mono(v))
 __device__ __forceinline__ float rank_value(u64 c) { return unmono(~(unsigned)(c >> 32)); }
 
 // ---- reductions over a workgroup of NT threads (red: NT / 64 words of LDS; every call starts with a barrier) ---------------------
+// Within a wave by data-parallel moves (shifts by 1, 2, 4, 8 inside a row of 16 lanes, then the rows' last lanes handed on): six dependent
+// steps of a few cycles instead of six trips through LDS.  The whole wave's result is in lane 63.
+template <int CTRL, int ROWS> __device__ __forceinline__ u64 dpp_u64(u64 other, u64 v) {       // `other` where there is no source lane
+    const unsigned lo = __builtin_amdgcn_update_dpp((unsigned)other, (unsigned)v, CTRL, ROWS, 0xF, false);
+    const unsigned hi = __builtin_amdgcn_update_dpp((unsigned)(other >> 32), (unsigned)(v >> 32), CTRL, ROWS, 0xF, false);
+    return ((u64)hi << 32) | lo;
+}
+__device__ __forceinline__ u64 wave_scan(u64 v) {              // inclusive
+    v += dpp_u64<0x111, 0xF>(0, v); v += dpp_u64<0x112, 0xF>(0, v); v += dpp_u64<0x114, 0xF>(0, v); v += dpp_u64<0x118, 0xF>(0, v);
+    v += dpp_u64<0x142, 0xA>(0, v); v += dpp_u64<0x143, 0xC>(0, v);
+    return v;
+}
+__device__ __forceinline__ u64 wave_min_63(u64 v) {
+    u64 x;
+    x = dpp_u64<0x111, 0xF>(~0ull, v); v = x < v ? x : v; x = dpp_u64<0x112, 0xF>(~0ull, v); v = x < v ? x : v;
+    x = dpp_u64<0x114, 0xF>(~0ull, v); v = x < v ? x : v; x = dpp_u64<0x118, 0xF>(~0ull, v); v = x < v ? x : v;
+    x = dpp_u64<0x142, 0xA>(~0ull, v); v = x < v ? x : v; x = dpp_u64<0x143, 0xC>(~0ull, v); v = x < v ? x : v;
+    return v;
+}
+template <int CTRL, int ROWS> __device__ __forceinline__ float dpp_max(float v) {
+    return fmaxf(v, __uint_as_float(__builtin_amdgcn_update_dpp(0xFF800000u, __float_as_uint(v), CTRL, ROWS, 0xF, false)));
+}
+__device__ __forceinline__ float wave_max_63(float v) {
+    v = dpp_max<0x111, 0xF>(v); v = dpp_max<0x112, 0xF>(v); v = dpp_max<0x114, 0xF>(v); v = dpp_max<0x118, 0xF>(v);
+    v = dpp_max<0x142, 0xA>(v); return dpp_max<0x143, 0xC>(v);
+}
 __device__ __forceinline__ u64 shfl_xor_u64(u64 v, int o) {
     const unsigned lo = __shfl_xor((unsigned)v, o, 64), hi = __shfl_xor((unsigned)(v >> 32), o, 64);
     return ((u64)hi << 32) | lo;
 }
-__device__ __forceinline__ u64 shfl_up_u64(u64 v, int o) {
-    const unsigned lo = __shfl_up((unsigned)v, o, 64), hi = __shfl_up((unsigned)(v >> 32), o, 64);
-    return ((u64)hi << 32) | lo;
-}
 template <int NT> __device__ __forceinline__ u64 block_min(u64 v, u64* red) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) { const u64 x = shfl_xor_u64(v, o); v = x < v ? x : v; }
+    v = wave_min_63(v);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = v;
     __syncthreads();
     v = red[0];
 #pragma unroll
     for (int i = 1; i < NT / 64; ++i) v = red[i] < v ? red[i] : v;
     return v;
 }
-template <int NT> __device__ __forceinline__ float block_max(float v, u64* red) {
-    v = wave_max(v);
+template <int NT> __device__ __forceinline__ float block_max(float v, u64* red, float* wave_top = nullptr) {
+    v = wave_max_63(v);
     float* r = (float*)red;
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 63) { r[threadIdx.x >> 6] = v; if (wave_top) wave_top[threadIdx.x >> 6] = v; }
     __syncthreads();
     v = r[0];
 #pragma unroll
@@ -114,9 +150,7 @@ template <int NT> __device__ __forceinline__ float block_max(float v, u64* red) 
 }
 // exclusive prefix over the threads; total = sum of all
 template <int NT> __device__ __forceinline__ u64 block_scan(u64 v, u64* red, u64& total) {
-    u64 s = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) { const u64 x = shfl_up_u64(s, o); if ((int)(threadIdx.x & 63) >= o) s += x; }
+    const u64 s = wave_scan(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = s;
     __syncthreads();
@@ -125,6 +159,22 @@ template <int NT> __device__ __forceinline__ u64 block_scan(u64 v, u64* red, u64
     for (int i = 0; i < NT / 64; ++i) { if (i < (int)(threadIdx.x >> 6)) before += red[i]; all += red[i]; }
     total = all;
     return before + s - v;
+}
+// two of them with one pair of barriers (red: twice as long)
+template <int NT> __device__ __forceinline__ void block_scan2(u64& v, u64& w, u64* red, u64& total_v, u64& total_w) {
+    const u64 s = wave_scan(v), t = wave_scan(w);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) { red[threadIdx.x >> 6] = s; red[NT / 64 + (threadIdx.x >> 6)] = t; }
+    __syncthreads();
+    u64 bv = 0, bw = 0, av = 0, aw = 0;
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) {
+        const u64 x = red[i], y = red[NT / 64 + i];
+        if (i < (int)(threadIdx.x >> 6)) { bv += x; bw += y; }
+        av += x; aw += y;
+    }
+    total_v = av; total_w = aw;
+    v = bv + s - v; w = bw + t - w;
 }
 
 // ---- weights ------------------------------------------------------------------------------------------------------------------------
@@ -142,6 +192,13 @@ __device__ __forceinline__ double expm1_64(double y) {
     p = __builtin_fma(p, y, 0.5); p = __builtin_fma(p, y, 1.0);
     return p * y;
 }
+// 2^38 (exp(f / 64) - 1), 0 <= f < 1, rounded to a whole number, as the low bits of 2^52 + x: the polynomial of degree 4 through the
+// Chebyshev nodes of [0, 1] (off by at most 1.6e-14 of exp)
+__device__ __forceinline__ u64 excess38(double f) {
+    double p = 688.02263742244156;
+    p = __builtin_fma(p, f, 174757.97387092107); p = __builtin_fma(p, f, 33554433.677011274); p = __builtin_fma(p, f, 4294967295.7903161);
+    return (u64)__double_as_longlong(__builtin_fma(p, f, 4503599627370496.0)) - 0x4330000000000000ull;
+}
 // x in [0, 2^51] rounded to a whole number: the low bits of 2^52 + x
 __device__ __forceinline__ u64 whole(double x) { return (u64)__double_as_longlong(x + 4503599627370496.0) - 0x4330000000000000ull; }
 struct Weigh {
@@ -153,10 +210,11 @@ struct Weigh {
     // 64 (z_max - z); SMP_BINS and more: no weight
     __device__ __forceinline__ double at(float v) const { return v == -INFINITY ? 1e300 : (top - (double)v) * s; }
     __device__ __forceinline__ u64 mass(double at) const {
-        if (!(at < (double)SMP_BINS)) return 0;
-        const int n = (int)at;
+        const double c = fmin(at, (double)(SMP_BINS - 1));     // (no branch: several tokens' chains interleave)
+        const int n = (int)c;
         const double e = exp_tab(*tab, n);
-        return whole(__builtin_fma(e, expm1_64((at - (double)n) * (-1.0 / 64.0)), e) * scale);
+        const u64 m = whole(__builtin_fma(e, expm1_64((c - (double)n) * (-1.0 / 64.0)), e) * scale);
+        return at < (double)SMP_BINS ? m : 0;
     }
     // what counts in the draw
     __device__ __forceinline__ u64 kept(float v, int i, u64 cut) const {
@@ -218,8 +276,9 @@ template <int NT, bool BY_MASS, class Each> __device__ __forceinline__ u64 selec
         });
         __syncthreads();
         const u64 mc = threadIdx.x < 256 ? L.c[threadIdx.x] : 0, mm = threadIdx.x < 256 ? L.m[threadIdx.x] : 0;
-        u64 tc, tm;
-        const u64 bc = before_c + block_scan<NT>(mc, red, tc), bm = before_m + block_scan<NT>(mm, red, tm);
+        u64 tc, tm, bc = mc, bm = mm;
+        block_scan2<NT>(bc, bm, red, tc, tm);
+        bc += before_c; bm += before_m;
         const u64 b = BY_MASS ? bm : bc, x = BY_MASS ? mm : mc, most = BY_MASS ? before_m + tm : before_c + tc, nd = need < most ? need : most;
         if (threadIdx.x < 256 && b < nd && b + x >= nd) { L.out[0] = threadIdx.x; L.out[1] = bc; L.out[2] = bm; }
         __syncthreads();
@@ -232,13 +291,15 @@ template <int NT, bool BY_MASS, class Each> __device__ __forceinline__ u64 selec
     }
     if (threadIdx.x == 0) L.n = 0;
     __syncthreads();
-    each([&](u64 r) { if (r >= lo && r <= hi) { const unsigned k = atomicAdd(&L.n, 1u); if (k < (unsigned)SelectLds<NT>::CAP) { L.list[k] = r; L.lm[k] = w.mass(w.at(rank_value(r))); } } });
+    each([&](u64 r) { if (r >= lo && r <= hi) { const unsigned k = atomicAdd(&L.n, 1u); if (k < (unsigned)SelectLds<NT>::CAP) L.list[k] = r; } });
     __syncthreads();
     n = (int)L.n;
     if (n == 0) { mass_to = before_m; return ~0ull; }
+    if ((int)threadIdx.x < n) L.lm[threadIdx.x] = w.mass(w.at(rank_value(L.list[threadIdx.x])));
+    __syncthreads();
     // g threads (a power of two, within a wave) share the comparisons of one token
     int g = 1;
-    while (g < 64 && n * g * 2 <= NT) g *= 2;
+    while (g < 64 && n > 16 * g && n * g * 2 <= NT) g *= 2;
     const int e = threadIdx.x / g, part = threadIdx.x & (g - 1);
     u64 c = 0, m = 0, mine = 0, own = 0;
     if (e < n) {
@@ -264,25 +325,30 @@ template <int NT, bool BY_MASS, class Each> __device__ __forceinline__ u64 selec
 // ---- one workgroup a row ---------------------------------------------------------------------------------------------------------------
 template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sample_row(SampleArgs a) {
     constexpr int E = Row<BF16>::E, NG = VPT / E, PER = SMP_BINS / NT;
-    __shared__ u64 red[NT / 64];
+    __shared__ u64 red[2 * (NT / 64)];
     __shared__ ExpTab tab;
     __shared__ u64 hist[SMP_BINS];
     __shared__ SelectLds<NT> L;
     __shared__ u64 zs[4];
     const int b = blockIdx.x, tid = threadIdx.x;
     const Row<BF16> row(a, b);
+    // thread t holds tokens t * VPT - o .. + VPT - 1
+    uint4 raw[NG];
+    row.load(tid * NG, 1, raw);
+    const int i0 = tid * VPT - row.o;
     const Settings st = settings_of(a, b);
     const float u = a.u[b];
-    // thread t holds tokens t * VPT - o .. + VPT - 1
+    exp_tab_init(tab);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) hist[tid + j * NT] = 0;
+    if (tid == 0) zs[0] = zs[1] = ~0ull;
     float v[VPT];
 #pragma unroll
-    for (int q = 0; q < NG; ++q) row.group(tid * NG + q, v + q * E);
-    const int i0 = tid * VPT - row.o;
-    exp_tab_init(tab);
+    for (int q = 0; q < NG; ++q) row.unpack(raw[q], v + q * E);
     float top = v[0];
 #pragma unroll
     for (int j = 1; j < VPT; ++j) top = fmaxf(top, v[j]);
-    top = block_max<NT>(top, red);
+    top = block_max<NT>(top, red);                         // (its barriers publish the tables and the empty histogram)
     if (top == -INFINITY) { if (tid == 0) sample_store(a, b, -1, -INFINITY); return; }
     if (st.greedy) {
         u64 best = ~0ull;
@@ -295,38 +361,32 @@ template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sa
     const Weigh w(&tab, top, st, a.frac);
     u64 cut = ~0ull;
     if (st.use_k || st.use_p) {
-#pragma unroll
-        for (int j = 0; j < PER; ++j) hist[tid * PER + j] = 0;
-        if (tid == 0) zs[0] = zs[1] = ~0ull;
-        __syncthreads();
-        // one word a token: 1 << 48 for the count, and 2^39 (1 - exp(-rest / 64)) of what the bin's edge exceeds it by (below 16384 / 64)
+        // one word a token: 1 << 48 for the count, and 2^38 (exp(rest / 64) - 1) of what it exceeds the bin's lower edge by (16384 tokens: below 2^46)
+        short bin[VPT];
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             const double at = w.at(v[j]);
-            if (at < (double)SMP_BINS) {
-                const int n = (int)at;
-                atomicAdd(&hist[n], (1ull << 48) + whole(-expm1_64((at - (double)n) * (-1.0 / 64.0)) * 0x1p39));
-            }
+            const int n = at < (double)SMP_BINS ? (int)at : SMP_BINS;
+            bin[j] = (short)n;
+            if (n < SMP_BINS) atomicAdd(&hist[n], (1ull << 48) + excess38((double)(n + 1) - at));
         }
         __syncthreads();
         u64 c[PER], m[PER], cs = 0, ms = 0;
+        const double edge = w.scale * exp_tab(tab, 1);     // (a bin's lower edge)
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const u64 h = hist[tid * PER + j];
             c[j] = h >> 48;
-            m[j] = (u64)(((double)c[j] - (double)(long long)(h & 0xFFFFFFFFFFFFull) * 0x1p-39) * exp_tab(tab, tid * PER + j) * w.scale + 0.5);
+            m[j] = (u64)(((double)(unsigned)c[j] + (double)(long long)(h & 0xFFFFFFFFFFFFull) * 0x1p-38) * exp_tab(tab, tid * PER + j) * edge + 0.5);
             cs += c[j]; ms += m[j];
         }
-        u64 call, mall;
-        const u64 cb = block_scan<NT>(cs, red, call), mb = block_scan<NT>(ms, red, mall);
+        u64 call, mall, cb = cs, mb = ms;
+        block_scan2<NT>(cb, mb, red, call, mall);
         // tokens of one bin, by rank
-        auto in_bin = [&](int bin) {
-            return [&, bin](auto f) {
+        auto in_bin = [&](int n) {
+            return [&, n](auto f) {
 #pragma unroll
-                for (int j = 0; j < VPT; ++j) {
-                    const double at = w.at(v[j]);
-                    if (at < (double)SMP_BINS && (int)at == bin) f(rank_of(v[j], i0 + j));
-                }
+                for (int j = 0; j < VPT; ++j) if (bin[j] == n) f(rank_of(v[j], i0 + j));
             };
         };
         u64 mass = mall;
@@ -348,7 +408,6 @@ template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sa
         if (st.use_p) {
             const u64 need = p_need(st.P, mass);
             u64 mm = mb;
-            __syncthreads();
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
                 if (tid * PER + j <= bk && mm < need && mm + m[j] >= need) { zs[1] = (u64)(tid * PER + j); zs[2] = c[j]; zs[3] = mm; }
@@ -398,7 +457,7 @@ struct ZoneRec {
     unsigned n;               // tokens in them
 };
 struct Chunk { double ref, g_top; u64 best; };                 // bin 0 holds tokens with floor((l - ref) 64 / T) = g_top
-struct Tile { u64 all, kept; float top; unsigned count; };     // in front of b0: mass, mass that min-p leaves, tokens; the tile's largest logit
+struct Tile { u64 all, kept; unsigned count, pad; float top[4]; };    // in front of b0: mass, mass that min-p leaves, tokens; largest logit of each quarter (a wave's)
 struct RowWs { u64* hist; Chunk* chunk; Tile* tile; ZoneRec* rec; u64* list; };
 static inline __host__ __device__ size_t ws_up(size_t n) { return (n + 15) & ~(size_t)15; }
 static inline __host__ __device__ size_t row_ws_bytes(int G, int tiles) {
@@ -416,7 +475,7 @@ __device__ __forceinline__ RowWs row_ws(const SampleArgs& a, int b) {
 }
 template <bool BF16> __global__ __launch_bounds__(256) void k_sample_hist(SampleArgs a) {
     constexpr int NT = 256, E = Row<BF16>::E, TG = SMP_TILE / E, NQ = TG / NT;
-    __shared__ u64 red[NT / 64];
+    __shared__ u64 red[2 * (NT / 64)];
     __shared__ u64 ring[SMP_BINS];
     const int chunk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
     const Row<BF16> row(a, b);
@@ -428,10 +487,14 @@ template <bool BF16> __global__ __launch_bounds__(256) void k_sample_hist(Sample
     double ref = 0.0, g_top = -INFINITY;                   // bin 0 of the ring, at place `head`; lower bins lie in front of it
     int head = 0;
     float bv = -INFINITY; int bi = 0;
+    const int place = (tid >> 6) * (TG / 4) + (tid & 63);   // a wave's quarter of the tile, 64 groups at a time
+    uint4 raw[NQ];                                         // (the next tile is on its way while one is counted)
+    row.load(t0 * TG + place, 64, raw);
     for (int t = t0; t < t1; ++t) {
         float v[NQ * E];
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) row.group(t * TG + q * NT + tid, v + q * E);
+        for (int q = 0; q < NQ; ++q) row.unpack(raw[q], v + q * E);
+        if (t + 1 < t1) row.load((t + 1) * TG + place, 64, raw);
         float mx = -INFINITY;
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
@@ -439,10 +502,9 @@ template <bool BF16> __global__ __launch_bounds__(256) void k_sample_hist(Sample
             for (int e = 0; e < E; ++e) {
                 const float x = v[q * E + e];
                 mx = fmaxf(mx, x);
-                if (x > bv) { bv = x; bi = (t * TG + q * NT + tid) * E - row.o + e; }       // (a thread's places ascend: the first of equals stays)
+                if (x > bv) { bv = x; bi = (t * TG + place + q * 64) * E - row.o + e; }     // (a thread's places ascend: the first of equals stays)
             }
-        mx = block_max<NT>(mx, red);
-        if (tid == 0) ws.tile[t].top = mx;
+        mx = block_max<NT>(mx, red, ws.tile[t].top);
         if (!bins || mx == -INFINITY) continue;
         const double g = floor(((double)mx - ref) * sc);
         if (!(g - g_top < (double)SMP_BINS)) {             // the first tokens, or all before lie below the window: start anew from here
@@ -460,7 +522,7 @@ template <bool BF16> __global__ __launch_bounds__(256) void k_sample_hist(Sample
 #pragma unroll
         for (int j = 0; j < NQ * E; ++j) {
             const double x = ((double)v[j] - ref) * sc, fl = floor(x), rel = g_top - fl;
-            if (rel < (double)SMP_BINS) atomicAdd(&ring[(head - (int)rel) & (SMP_BINS - 1)], (1ull << 48) + whole(expm1_64((x - fl) * (1.0 / 64.0)) * 0x1p38));
+            if (rel < (double)SMP_BINS) atomicAdd(&ring[(head - (int)rel) & (SMP_BINS - 1)], (1ull << 48) + excess38(x - fl));
         }
     }
     const u64 best = block_min<NT>(bv == -INFINITY ? ~0ull : rank_of(bv, bi), red);
@@ -469,9 +531,9 @@ template <bool BF16> __global__ __launch_bounds__(256) void k_sample_hist(Sample
 }
 
 #define SMP_TILES_MAX (E2T_SAMPLE_MAX_V / SMP_TILE + 1)
-__global__ __launch_bounds__(1024) void k_sample_zone(SampleArgs a) {
-    constexpr int NT = 1024, PER = SMP_BINS / NT;
-    __shared__ u64 red[NT / 64];
+__global__ __launch_bounds__(512) void k_sample_zone(SampleArgs a) {
+    constexpr int NT = 512, PER = SMP_BINS / NT;
+    __shared__ u64 red[2 * (NT / 64)];
     __shared__ ExpTab tab;
     __shared__ u64 zs[4];
     __shared__ double edge[SMP_TILES_MAX];
@@ -494,27 +556,39 @@ __global__ __launch_bounds__(1024) void k_sample_zone(SampleArgs a) {
     }
     if (tid == 0) zs[0] = zs[1] = ~0ull;
     __syncthreads();
-    u64 c[PER], m[PER], cs = 0, ms = 0;
+    // bin x: the chunks' bins that cover the row's bins x and x + 1, and in front the one that covers bin 0 alone
+    u64 c[PER] = {}, m[PER] = {}, cs = 0, ms = 0;
+    auto enter = [&](int j, u64 w, double e) {
+        c[j] += w >> 48;
+        m[j] += (u64)(((double)(unsigned)(w >> 48) + (double)(long long)(w & 0xFFFFFFFFFFFFull) * 0x1p-38) * e + 0.5);
+    };
+    constexpr int UN = 4;
+    for (int k0 = 0; k0 < a.G; k0 += UN) {                 // (loads of four chunks together)
+        u64 w[UN][PER];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        const int x = tid * PER + j;
-        u64 cn = 0, mass = 0;
-        for (int k = 0; k < a.G; ++k) {
-            const u64* h = ws.hist + (size_t)k * SMP_BINS;
-            const int r = x + 1 - shift[k];                // the chunk's bin that covers the row's bins x and x + 1
-            if (r >= 0 && r < SMP_BINS && x + 1 < SMP_BINS) {
-                const u64 w = h[r];
-                cn += w >> 48; mass += (u64)(((double)(w >> 48) + (double)(w & 0xFFFFFFFFFFFFull) * 0x1p-38) * exp_tab(tab, x + 1) * edge[k] + 0.5);
-            }
-            if (x == 0 && shift[k] == 0) {
-                const u64 w = h[0];
-                cn += w >> 48; mass += (u64)(((double)(w >> 48) + (double)(w & 0xFFFFFFFFFFFFull) * 0x1p-38) * edge[k] + 0.5);
+        for (int u = 0; u < UN; ++u) {
+            const int k = min(k0 + u, a.G - 1);
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const int r = tid * PER + j + 1 - shift[k];
+                w[u][j] = ws.hist[(size_t)k * SMP_BINS + min(max(r, 0), SMP_BINS - 1)];
             }
         }
-        c[j] = cn; m[j] = mass; cs += cn; ms += mass;
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const int k = min(k0 + u, a.G - 1);
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const int x = tid * PER + j, r = x + 1 - shift[k];
+                if (k0 + u < a.G && r >= 0 && r < SMP_BINS && x + 1 < SMP_BINS) enter(j, w[u][j], exp_tab(tab, x + 1) * edge[k]);
+            }
+        }
     }
-    u64 call, mall;
-    const u64 cb = block_scan<NT>(cs, red, call), mb = block_scan<NT>(ms, red, mall);
+    if (tid == 0) for (int k = 0; k < a.G; ++k) if (shift[k] == 0) enter(0, ws.hist[(size_t)k * SMP_BINS], edge[k]);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) { cs += c[j]; ms += m[j]; }
+    u64 call, mall, cb = cs, mb = ms;
+    block_scan2<NT>(cb, mb, red, call, mall);
     int bk = SMP_BINS;
     u64 least = mall;                                      // the top-k's mass is at least this
     const bool cut_k = st.use_k && (u64)st.k < call;
@@ -543,8 +617,9 @@ __global__ __launch_bounds__(1024) void k_sample_zone(SampleArgs a) {
 
 template <bool BF16> __global__ __launch_bounds__(256) void k_sample_gather(SampleArgs a) {
     constexpr int NT = 256, E = Row<BF16>::E, TG = SMP_TILE / E, NQ = TG / NT;
-    __shared__ u64 red[NT / 64];
+    __shared__ u64 red[2 * (NT / 64)];
     __shared__ ExpTab tab;
+    __shared__ unsigned base;
     const int t = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
     const Settings st = settings_of(a, b);
     const RowWs ws = row_ws(a, b);
@@ -553,69 +628,92 @@ template <bool BF16> __global__ __launch_bounds__(256) void k_sample_gather(Samp
     const Row<BF16> row(a, b);
     const Weigh w(&tab, rank_value(rec.best), st, a.frac);
     const double b0 = rec.b0, b1 = rec.b1;
-    const float mx = ws.tile[t].top;
-    if (!(floor(w.at(mx)) <= b1)) { if (tid == 0) { ws.tile[t].all = ws.tile[t].kept = 0; ws.tile[t].count = 0; } return; }
+    Tile& tile = ws.tile[t];
+    const float mx = fmaxf(fmaxf(tile.top[0], tile.top[1]), fmaxf(tile.top[2], tile.top[3]));
+    if (!(floor(w.at(mx)) <= b1)) { if (tid == 0) { tile.all = tile.kept = 0; tile.count = 0; } return; }
+    const int place = (tid >> 6) * (TG / 4) + (tid & 63);
+    const bool some = floor(w.at(tile.top[tid >> 6])) <= b1;               // (of this wave's quarter)
+    uint4 raw[NQ];
+    if (some) row.load(t * TG + place, 64, raw);
     exp_tab_init(tab);
     float v[NQ * E];
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) row.group(t * TG + q * NT + tid, v + q * E);
+    for (int j = 0; j < NQ * E; ++j) v[j] = -INFINITY;
+    if (some) {
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) row.unpack(raw[q], v + q * E);
+    }
     __syncthreads();
-    u64 s = 0, sk = 0;
-    unsigned cnt = 0;
+    u64 s = 0, sk = 0, cnt = 0;                            // cnt: tokens in front of the zone, and 2^32 for each in it
+    unsigned in = 0;
+    if (some)
 #pragma unroll
     for (int j = 0; j < NQ * E; ++j) {
         const double x = w.at(v[j]), bin = floor(x);
         if (bin < b0 && x < (double)SMP_BINS) { const u64 m = w.mass(x); s += m; ++cnt; if (x <= w.amax) sk += m; }
-        const bool in = bin >= b0 && bin <= b1;
-        const u64 vote = __ballot(in);
-        if (vote) {
-            unsigned base = 0;
-            const int lane = tid & 63, first = __ffsll((long long)vote) - 1;
-            if (lane == first) base = atomicAdd(&rec.n, (unsigned)__popcll(vote));
-            base = __shfl(base, first, 64);
-            if (in) {
-                const unsigned k = base + (unsigned)__popcll(vote & ((1ull << lane) - 1));
-                if (k < SMP_LIST) ws.list[k] = rank_of(v[j], (t * TG + (j / E) * NT + tid) * E - row.o + j % E);
-            }
-        }
+        if (bin >= b0 && bin <= b1) { in |= 1u << j; cnt += 1ull << 32; }
     }
     u64 all, kept, count;
-    block_scan<NT>(s, red, all);
-    block_scan<NT>(sk, red, kept);
-    block_scan<NT>((u64)cnt, red, count);
-    if (tid == 0) { ws.tile[t].all = all; ws.tile[t].kept = kept; ws.tile[t].count = (unsigned)count; }
+    const u64 before = block_scan<NT>(cnt, red, count);
+    if (tid == 0) base = count >> 32 ? atomicAdd(&rec.n, (unsigned)(count >> 32)) : 0;
+    block_scan2<NT>(s, sk, red, all, kept);                // (its barriers publish `base`)
+    unsigned k = base + (unsigned)(before >> 32);
+    for (; in; in &= in - 1, ++k) {
+        const int j = __ffs(in) - 1;
+        const int i = (t * TG + place + (j / E) * 64) * E - row.o + j % E;
+        if (k < SMP_LIST) ws.list[k] = rank_of(row.at(i), i);
+    }
+    if (tid == 0) { tile.all = all; tile.kept = kept; tile.count = (unsigned)count; }
 }
 
-template <bool BF16> __global__ __launch_bounds__(1024) void k_sample_draw(SampleArgs a) {
-    constexpr int NT = 1024, E = Row<BF16>::E, TG = SMP_TILE / E;
-    __shared__ u64 red[NT / 64];
+// The tokens of the zone once more by finer bins, SMP_SUB over its width, counted and weighed in one go: one of these holds the k-th token
+// and one the token that reaches p, and what is left to rank is a handful.
+#define SMP_SUB 1024
+template <bool BF16> __global__ __launch_bounds__(512) void k_sample_draw(SampleArgs a) {
+    constexpr int NT = 512, E = Row<BF16>::E, NG = SMP_TILE / NT / E, PER = SMP_SUB / NT, KEEP = 4;
+    __shared__ u64 red[2 * (NT / 64)];
     __shared__ ExpTab tab;
     __shared__ SelectLds<NT> L;
     __shared__ u64 tsum[SMP_TILES_MAX];
-    __shared__ u64 zs[2];
+    __shared__ u64 sub_m[SMP_SUB];
+    __shared__ unsigned sub_c[SMP_SUB];
+    __shared__ u64 zs[4];
     const int b = blockIdx.x, tid = threadIdx.x;
     const Settings st = settings_of(a, b);
     const RowWs ws = row_ws(a, b);
     const ZoneRec rec = *ws.rec;
+    const float u = a.u[b];
+    const Tile tile = ws.tile[min(tid, a.tiles - 1)];
     if (rec.best == ~0ull) { if (tid == 0) sample_store(a, b, -1, -INFINITY); return; }
     if (st.greedy) { if (tid == 0) sample_store(a, b, (int)(unsigned)rec.best, 0.0f); return; }
+    const bool cuts = rec.cut_k || rec.cut_p, in_list = rec.n <= SMP_LIST;
+    u64 mine[KEEP];                                        // this thread's part of the list
+#pragma unroll
+    for (int k = 0; k < KEEP; ++k) mine[k] = cuts && in_list && tid + k * NT < (int)rec.n ? ws.list[tid + k * NT] : ~0ull;
     const Row<BF16> row(a, b);
     exp_tab_init(tab);
     const Weigh w(&tab, rank_value(rec.best), st, a.frac);
-    if (tid < a.tiles) tsum[tid] = ws.tile[tid].kept;
-    __syncthreads();
+    if (tid < a.tiles) tsum[tid] = tile.kept;
     u64 cut = ~0ull;
-    if (rec.cut_k || rec.cut_p) {
+    if (cuts) {
+        for (int i = tid; i < SMP_SUB; i += NT) { sub_m[i] = 0; sub_c[i] = 0; }
+        if (tid == 0) zs[0] = zs[1] = ~0ull;
+        // counts and masses of all tiles in front of the zone
         u64 above, above_c;
-        block_scan<NT>(tid < a.tiles ? ws.tile[tid].all : 0, red, above);
-        block_scan<NT>(tid < a.tiles ? (u64)ws.tile[tid].count : 0, red, above_c);
-        // the tokens of the cut's bins: from the list, or, where they are more than it holds (a flat row), from the row itself
+        u64 ta = tid < a.tiles ? tile.all : 0, tc = tid < a.tiles ? (u64)tile.count : 0;
+        block_scan2<NT>(ta, tc, red, above, above_c);
+        // the tokens of the zone: from the list, or, where they are more than it holds (a flat row), from the row itself
         auto each = [&](auto f) {
-            if (rec.n <= SMP_LIST) { for (unsigned i = tid; i < rec.n; i += NT) f(ws.list[i]); }
-            else {
-                for (int q = tid; q < a.tiles * TG; q += NT) {
+            if (in_list) {
+#pragma unroll
+                for (int k = 0; k < KEEP; ++k) if (mine[k] != ~0ull) f(mine[k]);
+                for (int i = KEEP * NT + tid; i < (int)rec.n; i += NT) f(ws.list[i]);
+            } else {
+                for (int q = tid; q < a.tiles * (SMP_TILE / E); q += NT) {
+                    uint4 raw[1];
                     float v[E];
-                    row.group(q, v);
+                    row.load(q, 0, raw);
+                    row.unpack(raw[0], v);
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
                         const double bin = floor(w.at(v[e]));
@@ -624,44 +722,78 @@ template <bool BF16> __global__ __launch_bounds__(1024) void k_sample_draw(Sampl
                 }
             }
         };
+        const double fine = (double)SMP_SUB / (double)(rec.b1 + 1 - rec.b0);
+        auto sub_of = [&](u64 r) { return min((int)((w.at(rank_value(r)) - (double)rec.b0) * fine), SMP_SUB - 1); };
+        auto in_sub = [&](int i) { return [&, i](auto f) { each([&](u64 r) { if (sub_of(r) == i) f(r); }); }; };
+        each([&](u64 r) { const int i = sub_of(r); atomicAdd(&sub_c[i], 1u); atomicAdd(&sub_m[i], w.mass(w.at(rank_value(r)))); });
+        __syncthreads();
+        u64 c[PER], m[PER], cs = 0, ms = 0, x;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) { c[j] = sub_c[tid * PER + j]; m[j] = sub_m[tid * PER + j]; cs += c[j]; ms += m[j]; }
+        u64 cb = cs, mb = ms, xc;
+        block_scan2<NT>(cb, mb, red, xc, x);
+        cb += above_c; mb += above;
         u64 to, mass = rec.whole;
-        if (rec.cut_k) { cut = select_rank<NT, false>(each, ~0ull, (int)rec.n, (u64)st.k - above_c, w, L, red, to); mass = above + to; }
+        if (rec.cut_k) {
+            u64 cc = cb, mm = mb;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                if (cc < (u64)st.k && cc + c[j] >= (u64)st.k) { zs[0] = (u64)(tid * PER + j); zs[2] = cc; zs[3] = mm; }
+                cc += c[j]; mm += m[j];
+            }
+            __syncthreads();
+            const int i = (int)zs[0];
+            const u64 cf = zs[2], mf = zs[3];
+            cut = select_rank<NT, false>(in_sub(i), ~0ull, (int)sub_c[i], (u64)st.k - cf, w, L, red, to);
+            mass = mf + to;
+        }
         if (rec.cut_p) {
-            const u64 need = p_need(st.P, mass);
-            const u64 cp = select_rank<NT, true>(each, cut, (int)rec.n, need > above ? need - above : 1, w, L, red, to);
+            const u64 most = above + x;
+            const u64 nd = p_need(st.P, mass), need = nd > most ? most : nd > above ? nd : above + 1;
+            u64 mm = mb;
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                if (mm < need && mm + m[j] >= need) { zs[1] = (u64)(tid * PER + j); zs[2] = mm; }
+                mm += m[j];
+            }
+            __syncthreads();
+            const int i = (int)zs[1];
+            const u64 cp = select_rank<NT, true>(in_sub(i), cut, (int)sub_c[i], need - zs[2], w, L, red, to);
             cut = cp < cut ? cp : cut;
         }
         each([&](u64 r) {
             if (r <= cut) {
-                const double x = w.at(rank_value(r));
-                if (x <= w.amax) atomicAdd(&tsum[((int)(unsigned)r + row.o) / SMP_TILE], w.mass(x));
+                const double at = w.at(rank_value(r));
+                if (at <= w.amax) atomicAdd(&tsum[((int)(unsigned)r + row.o) / SMP_TILE], w.mass(at));
             }
         });
-        __syncthreads();
     }
+    __syncthreads();
     const u64 s = tid < a.tiles ? tsum[tid] : 0;
     u64 all;
     const u64 before = block_scan<NT>(s, red, all);
-    const u64 r = u_times(a.u[b], all);
+    const u64 r = u_times(u, all);
     if (before <= r && r < before + s) { zs[0] = (u64)tid; zs[1] = before; }
     __syncthreads();
     const int t = (int)zs[0];
     const u64 in_front = zs[1];
-    // the tile's tokens, in order: 4 (8) a thread
-    float v[E];
+    // the tile's tokens, in order: 8 a thread
+    uint4 raw[NG];
+    float v[NG * E];
+    const int q = (t * NT + tid) * NG, i0 = q * E - row.o;
+    row.load(q, 1, raw);
     u64 ms = 0;
-    const int q = t * TG + tid, i0 = q * E - row.o;
-    if (tid < TG) {
-        row.group(q, v);
 #pragma unroll
-        for (int e = 0; e < E; ++e) ms += w.kept(v[e], i0 + e, cut);
-    }
+    for (int n = 0; n < NG; ++n) row.unpack(raw[n], v + n * E);
+#pragma unroll
+    for (int e = 0; e < NG * E; ++e) ms += w.kept(v[e], i0 + e, cut);
     u64 x;
     u64 at = in_front + block_scan<NT>(ms, red, x);
-    if (tid < TG && at <= r && r < at + ms) {
+    if (at <= r && r < at + ms) {
         int pick = -1; float pv = 0.f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
+        for (int e = 0; e < NG * E; ++e) {
             const u64 m = w.kept(v[e], i0 + e, cut);
             if (pick < 0 && r < at + m) { pick = i0 + e; pv = v[e]; }
             at += m;
@@ -674,9 +806,12 @@ template <bool BF16> __global__ __launch_bounds__(1024) void k_sample_draw(Sampl
 #define SMP_ROW_MAX (16384 - 7)         // (a row may start up to seven elements behind a 16-byte boundary)
 static int frac_bits(int V) { int c = 0; while ((1ll << c) < V) ++c; return 62 - c < 50 ? 62 - c : 50; }
 static int long_tiles(int V) { return (V + 7 + SMP_TILE - 1) / SMP_TILE; }
-// chunks of a long row: enough workgroups for the chip (1024 in all, a tile each at least), at most SMP_CHUNK_TILES tiles in one
+// chunks of a long row: enough workgroups for the chip (1024 in all) but no more than k_sample_zone merges quickly (16, 16 KB each), at most
+// SMP_CHUNK_TILES tiles in one
 static int long_chunks(int B, int V) {
-    const int tiles = long_tiles(V), least = (tiles + SMP_CHUNK_TILES - 1) / SMP_CHUNK_TILES, want = (1024 + B - 1) / B;
+    const int tiles = long_tiles(V), least = (tiles + SMP_CHUNK_TILES - 1) / SMP_CHUNK_TILES;
+    int want = (1024 + B - 1) / B;
+    if (want > 16) want = 16;
     return want < least ? least : want > tiles ? tiles : want;
 }
 extern "C" size_t e2t_sample_ws_bytes(int B, int V) {
@@ -688,9 +823,9 @@ template <bool BF16> static void sample_go(SampleArgs& a, int B, void* stream) {
     else if (a.V <= SMP_ROW_MAX) hipLaunchKernelGGL((k_sample_row<BF16, 1024, 16>), dim3(B), dim3(1024), 0, ST, a);
     else {
         hipLaunchKernelGGL((k_sample_hist<BF16>), dim3(a.G, B), dim3(256), 0, ST, a);
-        hipLaunchKernelGGL(k_sample_zone, dim3(B), dim3(1024), 0, ST, a);
+        hipLaunchKernelGGL(k_sample_zone, dim3(B), dim3(512), 0, ST, a);
         hipLaunchKernelGGL((k_sample_gather<BF16>), dim3(a.tiles, B), dim3(256), 0, ST, a);
-        hipLaunchKernelGGL((k_sample_draw<BF16>), dim3(B), dim3(1024), 0, ST, a);
+        hipLaunchKernelGGL((k_sample_draw<BF16>), dim3(B), dim3(512), 0, ST, a);
     }
 }
 static int sample_launch(SampleArgs& a, int dtype, int B, const e2t_sample_cfg* cfg, void* ws, size_t ws_bytes, void* stream) {
