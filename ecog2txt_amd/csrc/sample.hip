@@ -8,8 +8,7 @@
 // a row over threads, waves or workgroups, and any order of atomics, gives the same sums, the same cut and the same token, bit for
 // bit.  fp32 sums would not do: over a flat vocabulary of 128 k tokens the borders between tokens lie 8e-6 of the whole apart and
 // 6e-8 of rounding moves the answer of one row in a hundred.
-// fp64 multiply-adds run at the rate of unpacked fp32 ones on this chip; the exponential is a product of two table entries (LDS) and
-// a polynomial of degree 6 over 1/64.
+// fp64 multiply-adds run at the rate of unpacked fp32 ones on this chip, and the exponential takes a table entry and a short polynomial.
 //
 // Finding the cut.  A histogram of 2048 bins of 1/64 in z (count and mass in one 64-bit LDS atomic) says in which bin the k-th token, or
 // p of the mass, lies; only that bin's tokens are ranked among themselves.
@@ -39,9 +38,12 @@ struct SampleArgs {
     char* ws; int G, tiles;                                    // long rows: workspace, chunks and tiles of a row
 };
 struct Settings { float T, P, M; int k; bool use_k, use_p, use_m, greedy; };
+// (all loads leave together: where there is no array, the row's u stands in as a readable place)
 __device__ __forceinline__ Settings settings_of(const SampleArgs& a, int b) {
+    const float t = *(a.t ? a.t + b : a.u + b), p = *(a.p ? a.p + b : a.u + b), m = *(a.m ? a.m + b : a.u + b);
+    const int k = *(a.k ? a.k + b : (const int*)a.u + b);
     Settings s;
-    s.T = a.t ? a.t[b] : a.t0; s.P = a.p ? a.p[b] : a.p0; s.M = a.m ? a.m[b] : a.m0; s.k = a.k ? a.k[b] : a.k0;
+    s.T = a.t ? t : a.t0; s.P = a.p ? p : a.p0; s.M = a.m ? m : a.m0; s.k = a.k ? k : a.k0;
     s.use_p = s.P < 1.0f; s.use_k = s.k > 0 && s.k < a.V; s.use_m = s.M > 0.0f; s.greedy = !(s.T > 0.0f);
     return s;
 }
@@ -178,19 +180,19 @@ template <int NT> __device__ __forceinline__ void block_scan2(u64& v, u64& w, u6
 }
 
 // ---- weights ------------------------------------------------------------------------------------------------------------------------
-// exp(-at / 64), at >= 0: exp(-floor(at) / 64) from two tables (of 32 and 64 entries), the rest from the series
-struct ExpTab { double a[32], b[64]; };
-__device__ __forceinline__ void exp_tab_init(ExpTab& t) {
+// 2^F exp(-at / 64), at >= 0: the nearest whole number's from a table in LDS (made as the product of two short ones; what lies 2048
+// or further down weighs nothing), the rest from the polynomial of degree 4 through the Chebyshev nodes of [-1/2, 1/2] (off by at most
+// 1.5e-14 of exp): about 18 instructions a token, and no branch between the tokens of a thread, so that their chains interleave.
+struct ExpTab { double e[SMP_BINS + 1], a[32], b[64]; };
+__device__ __forceinline__ void exp_tab_begin(ExpTab& t) {             // (a barrier between begin and fill, one between fill and use)
     if (threadIdx.x < 32) t.a[threadIdx.x] = exp(-(double)threadIdx.x);
     else if (threadIdx.x >= 64 && threadIdx.x < 128) t.b[threadIdx.x - 64] = exp(-(double)(threadIdx.x - 64) / 64.0);
 }
-__device__ __forceinline__ double exp_tab(const ExpTab& t, int n) { return t.a[n >> 6] * t.b[n & 63]; }
-// exp(y) - 1, |y| <= 1/64 (y^7 / 5040 = 4e-17)
-__device__ __forceinline__ double expm1_64(double y) {
-    double p = 1.0 / 720.0;
-    p = __builtin_fma(p, y, 1.0 / 120.0); p = __builtin_fma(p, y, 1.0 / 24.0); p = __builtin_fma(p, y, 1.0 / 6.0);
-    p = __builtin_fma(p, y, 0.5); p = __builtin_fma(p, y, 1.0);
-    return p * y;
+template <int NT> __device__ __forceinline__ void exp_tab_fill(ExpTab& t, int frac) {
+    const double scale = (double)(1ull << frac);
+#pragma unroll
+    for (int n = threadIdx.x; n < SMP_BINS; n += NT) t.e[n] = t.a[n >> 6] * t.b[n & 63] * scale;
+    if (threadIdx.x == 0) t.e[SMP_BINS] = 0.0;
 }
 // 2^38 (exp(f / 64) - 1), 0 <= f < 1, rounded to a whole number, as the low bits of 2^52 + x: the polynomial of degree 4 through the
 // Chebyshev nodes of [0, 1] (off by at most 1.6e-14 of exp)
@@ -199,22 +201,21 @@ __device__ __forceinline__ u64 excess38(double f) {
     p = __builtin_fma(p, f, 174757.97387092107); p = __builtin_fma(p, f, 33554433.677011274); p = __builtin_fma(p, f, 4294967295.7903161);
     return (u64)__double_as_longlong(__builtin_fma(p, f, 4503599627370496.0)) - 0x4330000000000000ull;
 }
-// x in [0, 2^51] rounded to a whole number: the low bits of 2^52 + x
-__device__ __forceinline__ u64 whole(double x) { return (u64)__double_as_longlong(x + 4503599627370496.0) - 0x4330000000000000ull; }
 struct Weigh {
     const ExpTab* tab; double top, s, scale, amax;             // s = 64 / T; amax: min-p as a bound of at
     __device__ __forceinline__ Weigh(const ExpTab* t, float top_, const Settings& st, int frac) {
         tab = t; top = top_; s = 64.0 / (double)st.T; scale = (double)(1ull << frac);
         amax = st.use_m ? -64.0 * log((double)fminf(st.M, 1.0f)) : INFINITY;
     }
+    __device__ __forceinline__ Weigh(const ExpTab* t, double top_, double s_, double amax_, int frac) : tab(t), top(top_), s(s_), scale((double)(1ull << frac)), amax(amax_) {}
     // 64 (z_max - z); SMP_BINS and more: no weight
     __device__ __forceinline__ double at(float v) const { return v == -INFINITY ? 1e300 : (top - (double)v) * s; }
     __device__ __forceinline__ u64 mass(double at) const {
-        const double c = fmin(at, (double)(SMP_BINS - 1));     // (no branch: several tokens' chains interleave)
-        const int n = (int)c;
-        const double e = exp_tab(*tab, n);
-        const u64 m = whole(__builtin_fma(e, expm1_64((c - (double)n) * (-1.0 / 64.0)), e) * scale);
-        return at < (double)SMP_BINS ? m : 0;
+        const double c = fmin(at, (double)SMP_BINS), t = c + 6755399441055744.0;          // (1.5 * 2^52: the low word is the nearest whole number)
+        const double f = c - (t - 6755399441055744.0);
+        double p = 2.483533181583589e-09;
+        p = __builtin_fma(p, f, -6.357853029268959e-07); p = __builtin_fma(p, f, 0.00012207031249960526); p = __builtin_fma(p, f, -0.015624999999848418); p = __builtin_fma(p, f, 1.0);
+        return (u64)__double_as_longlong(__builtin_fma(tab->e[(int)(unsigned)__double_as_longlong(t)], p, 4503599627370496.0)) - 0x4330000000000000ull;
     }
     // what counts in the draw
     __device__ __forceinline__ u64 kept(float v, int i, u64 cut) const {
@@ -338,7 +339,7 @@ template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sa
     const int i0 = tid * VPT - row.o;
     const Settings st = settings_of(a, b);
     const float u = a.u[b];
-    exp_tab_init(tab);
+    exp_tab_begin(tab);
 #pragma unroll
     for (int j = 0; j < PER; ++j) hist[tid + j * NT] = 0;
     if (tid == 0) zs[0] = zs[1] = ~0ull;
@@ -348,7 +349,7 @@ template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sa
     float top = v[0];
 #pragma unroll
     for (int j = 1; j < VPT; ++j) top = fmaxf(top, v[j]);
-    top = block_max<NT>(top, red);                         // (its barriers publish the tables and the empty histogram)
+    top = block_max<NT>(top, red);                         // (its barriers publish the short tables and the empty histogram)
     if (top == -INFINITY) { if (tid == 0) sample_store(a, b, -1, -INFINITY); return; }
     if (st.greedy) {
         u64 best = ~0ull;
@@ -359,6 +360,8 @@ template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sa
         return;
     }
     const Weigh w(&tab, top, st, a.frac);
+    exp_tab_fill<NT>(tab, a.frac);
+    __syncthreads();
     u64 cut = ~0ull;
     if (st.use_k || st.use_p) {
         // one word a token: 1 << 48 for the count, and 2^38 (exp(rest / 64) - 1) of what it exceeds the bin's lower edge by (16384 tokens: below 2^46)
@@ -372,12 +375,11 @@ template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sa
         }
         __syncthreads();
         u64 c[PER], m[PER], cs = 0, ms = 0;
-        const double edge = w.scale * exp_tab(tab, 1);     // (a bin's lower edge)
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const u64 h = hist[tid * PER + j];
             c[j] = h >> 48;
-            m[j] = (u64)(((double)(unsigned)c[j] + (double)(long long)(h & 0xFFFFFFFFFFFFull) * 0x1p-38) * exp_tab(tab, tid * PER + j) * edge + 0.5);
+            m[j] = (u64)(((double)(unsigned)c[j] + (double)(long long)(h & 0xFFFFFFFFFFFFull) * 0x1p-38) * tab.e[tid * PER + j + 1] + 0.5);
             cs += c[j]; ms += m[j];
         }
         u64 call, mall, cb = cs, mb = ms;
@@ -452,6 +454,9 @@ template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sa
 struct ZoneRec {
     u64 best;                 // rank of the row's first token (~0: none)
     u64 whole;                // mass of all tokens
+    double top, s, amax;      // the row's Weigh
+    float P; int k, greedy;   // and settings
+    float v_front, v_zone, v_min;   // as bounds of the logits: in front of b0; not behind b1; what min-p leaves
     int b0, b1;               // bins whose tokens are ranked one by one; in front of b0 everything is kept, behind b1 nothing
     int cut_k, cut_p;         // what is to be found in them
     unsigned n;               // tokens in them
@@ -472,6 +477,18 @@ __device__ __forceinline__ RowWs row_ws(const SampleArgs& a, int b) {
     r.rec = (ZoneRec*)p; p += ws_up(sizeof(ZoneRec));
     r.list = (u64*)p;
     return r;
+}
+// the lowest float whose at is below `bound` (or, closed, at most that): from the quotient's float, a step or two up or down
+__device__ __forceinline__ float lowest_float(const Weigh& w, double bound, bool closed) {
+    auto in = [&](unsigned o) { const double x = w.at(unmono(o)); return closed ? x <= bound : x < bound; };
+    const unsigned least = mono(-3.402823466e+38f), most = mono((float)w.top);
+    if (!in(most)) return INFINITY;                        // (no token at all)
+    if (in(least)) return unmono(least);
+    unsigned o = mono((float)fmax(w.top - bound / w.s, -3.402823466e+38));
+    o = o > most ? most : o;
+    for (int i = 0; i < 8 && o < most && !in(o); ++i) ++o;
+    for (int i = 0; i < 8 && o > least && in(o - 1); ++i) --o;
+    return unmono(o);
 }
 template <bool BF16> __global__ __launch_bounds__(256) void k_sample_hist(SampleArgs a) {
     constexpr int NT = 256, E = Row<BF16>::E, TG = SMP_TILE / E, NQ = TG / NT;
@@ -537,31 +554,42 @@ __global__ __launch_bounds__(512) void k_sample_zone(SampleArgs a) {
     __shared__ ExpTab tab;
     __shared__ u64 zs[4];
     __shared__ double edge[SMP_TILES_MAX];
+    __shared__ u64 bin_m[SMP_BINS], first_m;
+    __shared__ unsigned bin_c[SMP_BINS], first_c;
     __shared__ int shift[SMP_TILES_MAX];
     const int b = blockIdx.x, tid = threadIdx.x;
     const Settings st = settings_of(a, b);
     const RowWs ws = row_ws(a, b);
     ZoneRec& rec = *ws.rec;
-    exp_tab_init(tab);
+    exp_tab_begin(tab);
     u64 best = tid < a.G ? ws.chunk[tid].best : ~0ull;
     best = block_min<NT>(best, red);
-    if (tid == 0) { rec.best = best; rec.n = 0; rec.whole = 0; rec.cut_k = rec.cut_p = 0; rec.b0 = SMP_BINS + 1; rec.b1 = SMP_BINS; }
+    const Weigh w(&tab, rank_value(best), st, a.frac);
+    if (tid == 0) {
+        rec.best = best; rec.n = 0; rec.whole = 0; rec.cut_k = rec.cut_p = 0; rec.b0 = SMP_BINS + 1; rec.b1 = SMP_BINS;
+        rec.top = w.top; rec.s = w.s; rec.amax = w.amax; rec.P = st.P; rec.k = st.k; rec.greedy = st.greedy;
+        if (best != ~0ull && !st.greedy) {
+            rec.v_front = rec.v_zone = lowest_float(w, (double)SMP_BINS, false);
+            rec.v_min = w.amax < (double)SMP_BINS ? lowest_float(w, w.amax, true) : rec.v_front;
+        }
+    }
     if (best == ~0ull || st.greedy || (!st.use_k && !st.use_p)) return;
+    exp_tab_fill<NT>(tab, a.frac);
     if (tid < a.G) {
         const Chunk c = ws.chunk[tid];
         // the chunk's bin 0 lies at d .. of the row's units (>= 0: the row's largest is no smaller than the chunk's)
         const double d = c.best == ~0ull ? 1e300 : fmax(((double)rank_value(best) - c.ref) * (64.0 / (double)st.T) - c.g_top, 0.0), fl = floor(d);
         shift[tid] = fl < (double)SMP_BINS ? (int)fl : SMP_BINS;
-        edge[tid] = fl < (double)SMP_BINS ? exp((d - fl) * (-1.0 / 64.0)) * (double)(1ull << a.frac) : 0.0;
+        edge[tid] = fl < (double)SMP_BINS ? exp((d - fl) * (-1.0 / 64.0)) : 0.0;
     }
-    if (tid == 0) zs[0] = zs[1] = ~0ull;
+    if (tid == 0) { zs[0] = zs[1] = ~0ull; first_m = 0; first_c = 0; }
     __syncthreads();
     // bin x: the chunks' bins that cover the row's bins x and x + 1, and in front the one that covers bin 0 alone
-    u64 c[PER] = {}, m[PER] = {}, cs = 0, ms = 0;
-    auto enter = [&](int j, u64 w, double e) {
-        c[j] += w >> 48;
-        m[j] += (u64)(((double)(unsigned)(w >> 48) + (double)(long long)(w & 0xFFFFFFFFFFFFull) * 0x1p-38) * e + 0.5);
+    auto value = [](u64 w) {                               // count + excess of a word
+        return __builtin_fma((double)(unsigned)((w >> 32) & 0xFFFFu), 0x1p-6, __builtin_fma((double)(unsigned)w, 0x1p-38, (double)(unsigned)(w >> 48)));
     };
+    unsigned cn[PER] = {};
+    double ms0[PER] = {};
     constexpr int UN = 4;
     for (int k0 = 0; k0 < a.G; k0 += UN) {                 // (loads of four chunks together)
         u64 w[UN][PER];
@@ -569,24 +597,35 @@ __global__ __launch_bounds__(512) void k_sample_zone(SampleArgs a) {
         for (int u = 0; u < UN; ++u) {
             const int k = min(k0 + u, a.G - 1);
 #pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                const int r = tid * PER + j + 1 - shift[k];
-                w[u][j] = ws.hist[(size_t)k * SMP_BINS + min(max(r, 0), SMP_BINS - 1)];
-            }
+            for (int j = 0; j < PER; ++j) w[u][j] = ws.hist[(size_t)k * SMP_BINS + min(max(j * NT + tid + 1 - shift[k], 0), SMP_BINS - 1)];
         }
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
             const int k = min(k0 + u, a.G - 1);
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
-                const int x = tid * PER + j, r = x + 1 - shift[k];
-                if (k0 + u < a.G && r >= 0 && r < SMP_BINS && x + 1 < SMP_BINS) enter(j, w[u][j], exp_tab(tab, x + 1) * edge[k]);
+                const int x = j * NT + tid, r = x + 1 - shift[k];
+                const bool on = k0 + u < a.G && r >= 0 && x + 1 < SMP_BINS;
+                cn[j] += on ? (unsigned)(w[u][j] >> 48) : 0;
+                ms0[j] = __builtin_fma(value(w[u][j]), on ? edge[k] : 0.0, ms0[j]);
             }
         }
     }
-    if (tid == 0) for (int k = 0; k < a.G; ++k) if (shift[k] == 0) enter(0, ws.hist[(size_t)k * SMP_BINS], edge[k]);
+    if (tid < a.G && shift[tid] == 0) {
+        const u64 w = ws.hist[(size_t)tid * SMP_BINS];
+        atomicAdd(&first_c, (unsigned)(w >> 48));
+        atomicAdd(&first_m, (u64)(value(w) * edge[tid] * tab.e[0] + 0.5));
+    }
 #pragma unroll
-    for (int j = 0; j < PER; ++j) { cs += c[j]; ms += m[j]; }
+    for (int j = 0; j < PER; ++j) { bin_c[j * NT + tid] = cn[j]; bin_m[j * NT + tid] = (u64)(ms0[j] * tab.e[j * NT + tid + 1] + 0.5); }
+    __syncthreads();
+    u64 c[PER], m[PER], cs = 0, ms = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        c[j] = bin_c[tid * PER + j]; m[j] = bin_m[tid * PER + j];
+        if (tid == 0 && j == 0) { c[j] += first_c; m[j] += first_m; }
+        cs += c[j]; ms += m[j];
+    }
     u64 call, mall, cb = cs, mb = ms;
     block_scan2<NT>(cb, mb, red, call, mall);
     int bk = SMP_BINS;
@@ -612,47 +651,68 @@ __global__ __launch_bounds__(512) void k_sample_zone(SampleArgs a) {
         __syncthreads();
         if (zs[1] != ~0ull) b0 = min(bk, (int)zs[1]);
     }
+    if (tid == 64 && b0 < SMP_BINS) rec.v_front = lowest_float(w, (double)b0, false);
+    if (tid == 128 && b0 < SMP_BINS) rec.v_zone = lowest_float(w, (double)((cut_k ? bk : b0) + 2), false);
     if (tid == 0 && b0 < SMP_BINS) { rec.whole = mall; rec.b0 = b0; rec.b1 = (cut_k ? bk : b0) + 1; rec.cut_k = cut_k; rec.cut_p = st.use_p; }
 }
 
-template <bool BF16> __global__ __launch_bounds__(256) void k_sample_gather(SampleArgs a) {
+template <bool BF16> __global__ __launch_bounds__(256, 6) void k_sample_gather(SampleArgs a) {
     constexpr int NT = 256, E = Row<BF16>::E, TG = SMP_TILE / E, NQ = TG / NT;
     __shared__ u64 red[2 * (NT / 64)];
     __shared__ ExpTab tab;
     __shared__ unsigned base;
     const int t = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-    const Settings st = settings_of(a, b);
     const RowWs ws = row_ws(a, b);
     ZoneRec& rec = *ws.rec;
-    if (st.greedy || rec.best == ~0ull) return;
-    const Row<BF16> row(a, b);
-    const Weigh w(&tab, rank_value(rec.best), st, a.frac);
-    const double b0 = rec.b0, b1 = rec.b1;
     Tile& tile = ws.tile[t];
     const float mx = fmaxf(fmaxf(tile.top[0], tile.top[1]), fmaxf(tile.top[2], tile.top[3]));
-    if (!(floor(w.at(mx)) <= b1)) { if (tid == 0) { tile.all = tile.kept = 0; tile.count = 0; } return; }
+    if (rec.greedy || rec.best == ~0ull) return;
+    const Row<BF16> row(a, b);
+    const Weigh w(&tab, rec.top, rec.s, rec.amax, a.frac);
+    const float v_front = rec.v_front, v_zone = rec.v_zone, v_min = rec.v_min;
+    if (!(mx >= v_zone)) { if (tid == 0) { tile.all = tile.kept = 0; tile.count = 0; } return; }
     const int place = (tid >> 6) * (TG / 4) + (tid & 63);
-    const bool some = floor(w.at(tile.top[tid >> 6])) <= b1;               // (of this wave's quarter)
+    const bool some = tile.top[tid >> 6] >= v_zone;        // (of this wave's quarter)
     uint4 raw[NQ];
     if (some) row.load(t * TG + place, 64, raw);
-    exp_tab_init(tab);
-    float v[NQ * E];
-#pragma unroll
-    for (int j = 0; j < NQ * E; ++j) v[j] = -INFINITY;
-    if (some) {
-#pragma unroll
-        for (int q = 0; q < NQ; ++q) row.unpack(raw[q], v + q * E);
-    }
+    exp_tab_begin(tab);
+    __syncthreads();
+    exp_tab_fill<NT>(tab, a.frac);
     __syncthreads();
     u64 s = 0, sk = 0, cnt = 0;                            // cnt: tokens in front of the zone, and 2^32 for each in it
     unsigned in = 0;
-    if (some)
+    const bool cuts = rec.cut_k || rec.cut_p, mp = rec.amax < INFINITY;
+    if (some) {
+        float v[NQ * E];
 #pragma unroll
-    for (int j = 0; j < NQ * E; ++j) {
-        const double x = w.at(v[j]), bin = floor(x);
-        if (bin < b0 && x < (double)SMP_BINS) { const u64 m = w.mass(x); s += m; ++cnt; if (x <= w.amax) sk += m; }
-        if (bin >= b0 && bin <= b1) { in |= 1u << j; cnt += 1ull << 32; }
+        for (int q = 0; q < NQ; ++q) row.unpack(raw[q], v + q * E);
+        if (!cuts && !mp) {
+#pragma unroll
+            for (int j = 0; j < NQ * E; ++j) s += w.mass(w.at(v[j]));
+        } else {
+#pragma unroll
+            for (int j0 = 0; j0 < NQ * E; j0 += 4) {
+                bool any = false;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const float x = v[j0 + c];
+                    const bool front = x >= v_front;
+                    if (x >= v_zone && !front) { in |= 1u << (j0 + c); cnt += 1ull << 32; }
+                    cnt += front;
+                    any |= front;
+                }
+                if (__any(any)) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const float x = v[j0 + c];
+                        const u64 m = x >= v_front ? w.mass(w.at(x)) : 0;
+                        s += m; sk += x >= v_min ? m : 0;
+                    }
+                }
+            }
+        }
     }
+    if (!mp) sk = s;
     u64 all, kept, count;
     const u64 before = block_scan<NT>(cnt, red, count);
     if (tid == 0) base = count >> 32 ? atomicAdd(&rec.n, (unsigned)(count >> 32)) : 0;
@@ -679,21 +739,23 @@ template <bool BF16> __global__ __launch_bounds__(512) void k_sample_draw(Sample
     __shared__ unsigned sub_c[SMP_SUB];
     __shared__ u64 zs[4];
     const int b = blockIdx.x, tid = threadIdx.x;
-    const Settings st = settings_of(a, b);
     const RowWs ws = row_ws(a, b);
     const ZoneRec rec = *ws.rec;
     const float u = a.u[b];
     const Tile tile = ws.tile[min(tid, a.tiles - 1)];
     if (rec.best == ~0ull) { if (tid == 0) sample_store(a, b, -1, -INFINITY); return; }
-    if (st.greedy) { if (tid == 0) sample_store(a, b, (int)(unsigned)rec.best, 0.0f); return; }
+    if (rec.greedy) { if (tid == 0) sample_store(a, b, (int)(unsigned)rec.best, 0.0f); return; }
     const bool cuts = rec.cut_k || rec.cut_p, in_list = rec.n <= SMP_LIST;
     u64 mine[KEEP];                                        // this thread's part of the list
 #pragma unroll
     for (int k = 0; k < KEEP; ++k) mine[k] = cuts && in_list && tid + k * NT < (int)rec.n ? ws.list[tid + k * NT] : ~0ull;
     const Row<BF16> row(a, b);
-    exp_tab_init(tab);
-    const Weigh w(&tab, rank_value(rec.best), st, a.frac);
+    exp_tab_begin(tab);
+    __syncthreads();
+    exp_tab_fill<NT>(tab, a.frac);
+    const Weigh w(&tab, rec.top, rec.s, rec.amax, a.frac);
     if (tid < a.tiles) tsum[tid] = tile.kept;
+    __syncthreads();
     u64 cut = ~0ull;
     if (cuts) {
         for (int i = tid; i < SMP_SUB; i += NT) { sub_m[i] = 0; sub_c[i] = 0; }
@@ -716,15 +778,24 @@ template <bool BF16> __global__ __launch_bounds__(512) void k_sample_draw(Sample
                     row.unpack(raw[0], v);
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
-                        const double bin = floor(w.at(v[e]));
-                        if (bin >= (double)rec.b0 && bin <= (double)rec.b1) f(rank_of(v[e], q * E - row.o + e));
+                        if (v[e] >= rec.v_zone && v[e] < rec.v_front) f(rank_of(v[e], q * E - row.o + e));
                     }
                 }
             }
         };
         const double fine = (double)SMP_SUB / (double)(rec.b1 + 1 - rec.b0);
         auto sub_of = [&](u64 r) { return min((int)((w.at(rank_value(r)) - (double)rec.b0) * fine), SMP_SUB - 1); };
-        auto in_sub = [&](int i) { return [&, i](auto f) { each([&](u64 r) { if (sub_of(r) == i) f(r); }); }; };
+        int my_sub[KEEP];
+#pragma unroll
+        for (int k = 0; k < KEEP; ++k) my_sub[k] = mine[k] != ~0ull ? sub_of(mine[k]) : -1;
+        auto in_sub = [&](int i) {
+            return [&, i](auto f) {
+                if (rec.n <= KEEP * NT) {
+#pragma unroll
+                    for (int k = 0; k < KEEP; ++k) if (my_sub[k] == i) f(mine[k]);
+                } else each([&](u64 r) { if (sub_of(r) == i) f(r); });
+            };
+        };
         each([&](u64 r) { const int i = sub_of(r); atomicAdd(&sub_c[i], 1u); atomicAdd(&sub_m[i], w.mass(w.at(rank_value(r)))); });
         __syncthreads();
         u64 c[PER], m[PER], cs = 0, ms = 0, x;
@@ -738,18 +809,18 @@ template <bool BF16> __global__ __launch_bounds__(512) void k_sample_draw(Sample
             u64 cc = cb, mm = mb;
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
-                if (cc < (u64)st.k && cc + c[j] >= (u64)st.k) { zs[0] = (u64)(tid * PER + j); zs[2] = cc; zs[3] = mm; }
+                if (cc < (u64)rec.k && cc + c[j] >= (u64)rec.k) { zs[0] = (u64)(tid * PER + j); zs[2] = cc; zs[3] = mm; }
                 cc += c[j]; mm += m[j];
             }
             __syncthreads();
             const int i = (int)zs[0];
             const u64 cf = zs[2], mf = zs[3];
-            cut = select_rank<NT, false>(in_sub(i), ~0ull, (int)sub_c[i], (u64)st.k - cf, w, L, red, to);
+            cut = select_rank<NT, false>(in_sub(i), ~0ull, (int)sub_c[i], (u64)rec.k - cf, w, L, red, to);
             mass = mf + to;
         }
         if (rec.cut_p) {
             const u64 most = above + x;
-            const u64 nd = p_need(st.P, mass), need = nd > most ? most : nd > above ? nd : above + 1;
+            const u64 nd = p_need(rec.P, mass), need = nd > most ? most : nd > above ? nd : above + 1;
             u64 mm = mb;
             __syncthreads();
 #pragma unroll
@@ -803,7 +874,7 @@ template <bool BF16> __global__ __launch_bounds__(512) void k_sample_draw(Sample
 }
 
 // ---- entry points -----------------------------------------------------------------------------------------------------------------------
-#define SMP_ROW_MAX (16384 - 7)         // (a row may start up to seven elements behind a 16-byte boundary)
+#define SMP_ROW_MAX (8192 - 7)          // (a row may start up to seven elements behind a 16-byte boundary)
 static int frac_bits(int V) { int c = 0; while ((1ll << c) < V) ++c; return 62 - c < 50 ? 62 - c : 50; }
 static int long_tiles(int V) { return (V + 7 + SMP_TILE - 1) / SMP_TILE; }
 // chunks of a long row: enough workgroups for the chip (1024 in all) but no more than k_sample_zone merges quickly (16, 16 KB each), at most
@@ -819,8 +890,7 @@ extern "C" size_t e2t_sample_ws_bytes(int B, int V) {
 }
 template <bool BF16> static void sample_go(SampleArgs& a, int B, void* stream) {
     if (a.V <= 2048 - 7) hipLaunchKernelGGL((k_sample_row<BF16, 256, 8>), dim3(B), dim3(256), 0, ST, a);
-    else if (a.V <= 8192 - 7) hipLaunchKernelGGL((k_sample_row<BF16, 512, 16>), dim3(B), dim3(512), 0, ST, a);
-    else if (a.V <= SMP_ROW_MAX) hipLaunchKernelGGL((k_sample_row<BF16, 1024, 16>), dim3(B), dim3(1024), 0, ST, a);
+    else if (a.V <= SMP_ROW_MAX) hipLaunchKernelGGL((k_sample_row<BF16, 512, 16>), dim3(B), dim3(512), 0, ST, a);
     else {
         hipLaunchKernelGGL((k_sample_hist<BF16>), dim3(a.G, B), dim3(256), 0, ST, a);
         hipLaunchKernelGGL(k_sample_zone, dim3(B), dim3(512), 0, ST, a);
