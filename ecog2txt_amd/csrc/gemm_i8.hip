@@ -5,6 +5,7 @@
 // The sum is exact (int32, K <= 131071); it is rounded once to fp32, scaled, biased and rounded to the output type.
 #include "common.h"
 #include "ecog2txt_hip.h"
+#include <atomic>
 #include <math.h>
 
 #define ST ((hipStream_t)stream)
@@ -390,6 +391,17 @@ __global__ __launch_bounds__(64 * NWV) void k_gemm_i8_rows(I8Args p) {
     }
 }
 
+// Kernels above 64 KiB of LDS ask for it before their first launch on each device (`done`: a bit a device; a race sets the same attribute twice).
+static int i8_lds(const void* kern, size_t lds, size_t most, std::atomic<unsigned long long>& done) {
+    if (lds <= 65536) return E2T_OK;
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) { e2t_set_error("%s:%d: no current device", __FILE__, __LINE__); return E2T_ERR_HIP; }
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return E2T_OK;
+    if (hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)most) != hipSuccess) { e2t_set_error("%s:%d: LDS size", __FILE__, __LINE__); return E2T_ERR_HIP; }
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return E2T_OK;
+}
 template <int BM, int BN, int WM, int WN, int NS, int KS, int WGS, bool QUARTERS> static int i8_tile_launch(I8Args p, void* stream) {
     constexpr int lds = (BM + BN) * 64 * NS * KS + (BM + 2 * BN) * 4;
     static_assert(lds * WGS <= 160 * 1024, "LDS");
@@ -399,28 +411,16 @@ template <int BM, int BN, int WM, int WN, int NS, int KS, int WGS, bool QUARTERS
     if (QUARTERS) { const int left = (int)(W % 256); if (W > 256 && left <= I8_QUARTERED) p.full = (int)W - left; }
     const unsigned grid = (unsigned)(p.full + (W - p.full) * 4);
     auto kern = k_gemm_i8_tile<BM, BN, WM, WN, NS, KS, WGS, QUARTERS>;
-    if (lds > 65536) {
-        static bool done;          // (idempotent: a race sets the same attribute twice)
-        if (!done) {
-            if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) { e2t_set_error("%s:%d: LDS size", __FILE__, __LINE__); return E2T_ERR_HIP; }
-            done = true;
-        }
-    }
+    static std::atomic<unsigned long long> done;
+    if (int rc = i8_lds((const void*)kern, lds, lds, done)) return rc;
     hipLaunchKernelGGL(kern, dim3(grid), dim3(64 * WM * WN * KS), lds, ST, p);
     E2T_LAUNCH_CHECK(); return E2T_OK;
-}
-static int i8_lds(const void* kern, size_t lds, size_t most, bool& done) {      // (idempotent: a race sets the same attribute twice)
-    if (lds > 65536 && !done) {
-        if (hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)most) != hipSuccess) { e2t_set_error("%s:%d: LDS size", __FILE__, __LINE__); return E2T_ERR_HIP; }
-        done = true;
-    }
-    return E2T_OK;
 }
 template <int MT, int NTL, int NWV, int D> static int i8_rows_launch(const I8Args& p, void* stream) {
     const dim3 grid((p.N + NTL * 16 - 1) / (NTL * 16), (p.M + MT * 16 - 1) / (MT * 16));
     E2T_CHECK_ARG(grid.y <= 65535);
     constexpr size_t lds = NWV * D * (MT + NTL) * 1024;
-    static bool done;
+    static std::atomic<unsigned long long> done;
     auto kern = k_gemm_i8_rows<MT, NTL, NWV, D, 0>;
     if (int rc = i8_lds((const void*)kern, lds, lds, done)) return rc;
     hipLaunchKernelGGL(kern, grid, dim3(64 * NWV), lds, ST, p);
@@ -475,7 +475,7 @@ static int i8_launch(const I8Args& p, void* stream) {
 template <int NTL, int NWV, int D> static int i8_fused_launch(const I8Args& p, void* stream) {
     const dim3 grid((p.N + NTL * 16 - 1) / (NTL * 16));
     const size_t lds = NWV * D * NTL * 1024 + (size_t)p.M * (p.S * 64 + 16);
-    static bool done[2];
+    static std::atomic<unsigned long long> done[2];
     auto kern = p.xbf16 ? k_gemm_i8_rows<1, NTL, NWV, D, 2> : k_gemm_i8_rows<1, NTL, NWV, D, 1>;
     if (int rc = i8_lds((const void*)kern, lds, 140 * 1024, done[p.xbf16])) return rc;
     hipLaunchKernelGGL(kern, grid, dim3(64 * NWV), lds, ST, p);
