@@ -165,6 +165,7 @@ class Seq2SeqEngine(PackingMixin, DecodingMixin):
         self._lstream = None
         self._dec_table = None          # decoding: the decoder's input projection of every token (decoding.py)
         self._dec_table_key, self._img_version, self._head_scratch = None, 0, None
+        self._proj_i8, self._proj_i8_key = None, None          # the vocabulary projection in 8 bits (decoding.py)
         self.small_batch_head_max = 2   # greedy decoding: the one-launch head (e2t_greedy_head_small) up to this many utterances
         self.launch_stream_on = bool(opt['launch_stream'])
         # (measured and dropped in rounds 1-2, DESIGN.md appendix: weight gradients on TWO side streams, the BPTT chain alone

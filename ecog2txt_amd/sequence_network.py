@@ -556,10 +556,12 @@ class SequenceNetwork:
         res = {k: (np.concatenate(v, axis=1 if k == 'final_RNN_state' else 0) if v else None) for k, v in out.items()}
         return res
 
-    def online_predictor(self, subjects, restore_epoch, targets_list=None, subject=None, max_length=None):
+    def online_predictor(self, subjects, restore_epoch, targets_list=None, subject=None, max_length=None, sampling=None):
         """predict(inputs) for one utterance [T,C] or a batch [B,T,C] of (zero-padded) ECoG: greedy word sequences
         from the restored EMA weights -- the device-resident counterpart of the reference's SavedModel predictor
-        (trainers.py:925-949).  With targets_list the hypotheses come back as strings, else as token-id arrays."""
+        (trainers.py:925-949).  With targets_list the hypotheses come back as strings, else as token-id arrays.
+        sampling: a dict of temperature, top_k, top_p, min_p, int8_projection (the engine's sample_decode) and seed: words are drawn, from a
+        generator of the predictor's own, in place of the greedy ones."""
         import torch
         eng = self._get_engine(subjects)
         self._restore(eng, restore_epoch, None)
@@ -567,6 +569,11 @@ class SequenceNetwork:
         N = eng.spec.decimation
         L = int(max_length or self.max_hyp_length)
         eng.pack('ema')
+        if sampling is not None:
+            draw = dict(sampling)
+            numbers = torch.Generator(device=eng.device).manual_seed(int(draw.pop('seed', self.seed)))
+            if not set(draw) <= {'temperature', 'top_k', 'top_p', 'min_p', 'int8_projection'}:
+                raise ValueError('sampling: unknown settings %s' % sorted(set(draw) - {'temperature', 'top_k', 'top_p', 'min_p', 'int8_projection'}))
 
         def predict(inputs):
             x = np.asarray(inputs, np.float32)
@@ -577,7 +584,11 @@ class SequenceNetwork:
             ws['X'].zero_()
             ws['X'][:, :x.shape[1]].copy_(torch.from_numpy(np.ascontiguousarray(x)))
             ws['Y'].zero_()
-            hyp = eng.greedy_decode(ws, which='ema').cpu().numpy()
+            if sampling is not None:
+                hyp, _ = eng.sample_decode(ws, torch.rand(L, B, generator=numbers, device=eng.device), which='ema', **draw)
+            else:
+                hyp = eng.greedy_decode(ws, which='ema')
+            hyp = hyp.cpu().numpy()
             eng.check_sync(ws)
             return target_inds_to_sequences(hyp, list(targets_list)) if targets_list is not None else hyp
         return predict

@@ -300,16 +300,16 @@ class MultiSubjectTrainer:
         return self.net.restore_and_get_internal_activations(self.ecog_subjects, self.restore_epoch,
                                                               data_partition='validation')
 
-    def construct_online_predictor(self, targets_list=None, subject=None, max_length=None):
+    def construct_online_predictor(self, targets_list=None, subject=None, max_length=None, sampling=None):
         """predict(inputs) -> hypotheses for raw ECoG [T,C] / [B,T,C] with the saved model (the reference builds this
         from a SavedModel export, trainers.py:925-949; here from this trainer's checkpoint).  targets_list defaults
-        to the decoder vocabulary, so the hypotheses are word strings."""
+        to the decoder vocabulary, so the hypotheses are word strings.  sampling: SequenceNetwork.online_predictor."""
         self.update_net_from_saved_model()
         subject = subject or self.ecog_subjects[-1]
         if targets_list is None:
             targets_list = list(subject.data_manifests['decoder_targets'].get_feature_list())
         return self.net.online_predictor(self.ecog_subjects, self.restore_epoch, targets_list=targets_list,
-                                         subject=subject, max_length=max_length)
+                                         subject=subject, max_length=max_length, sampling=sampling)
 
     def subject_to_table(self):
         import pandas as pd
