@@ -483,7 +483,7 @@ template <int NTL, int NWV, int D> static int i8_fused_launch(const I8Args& p, v
 }
 
 extern "C" int e2t_quant_rows_i8(const void* x, int dtype, long long ldx, int M, int K, int8_t* q, long long ldq, float* scale, void* stream) {
-    E2T_CHECK_ARG(x && q && scale && M > 0 && K > 0 && ldx >= K && (dtype == E2T_DT_F32 || dtype == E2T_DT_BF16));
+    E2T_CHECK_ARG(x && q && scale && M > 0 && M <= E2T_I8_MAX_ROWS && K > 0 && K < (1 << 30) && ldx >= K && (dtype == E2T_DT_F32 || dtype == E2T_DT_BF16));
     E2T_CHECK_ARG(ldq >= ((K + 63) & ~63) && (ldq & 15) == 0 && ((uintptr_t)q & 15) == 0 && ((uintptr_t)x & (dtype == E2T_DT_F32 ? 3 : 1)) == 0);
     const int vec = (((uintptr_t)x | (unsigned long long)(ldx * (dtype == E2T_DT_F32 ? 4 : 2))) & 15) == 0;
 #define QL(T, NC)                                                                                                                             \
@@ -500,7 +500,7 @@ extern "C" int e2t_quant_rows_i8(const void* x, int dtype, long long ldx, int M,
 }
 
 static int gemm_i8_check(const void* B, long long ldb, const float* sb, const void* C, long long ldc, int M, int N, int K, int flags) {
-    E2T_CHECK_ARG(B && sb && C && M > 0 && N > 0 && K > 0 && K <= E2T_I8_MAX_K);
+    E2T_CHECK_ARG(B && sb && C && M > 0 && M <= E2T_I8_MAX_ROWS && N > 0 && N <= E2T_I8_MAX_ROWS && K > 0 && K <= E2T_I8_MAX_K);
     const long long K64 = ((long long)K + 63) & ~63ll;
     E2T_CHECK_ARG(ldb <= E2T_I8_MAX_LD && ldb >= K64 && (ldb & 15) == 0 && ldc >= N && ((uintptr_t)B & 15) == 0);
     E2T_CHECK_ARG((flags & ~(E2T_GEMM_RELU | E2T_GEMM_OUT_BF16)) == 0 && ((uintptr_t)C & ((flags & E2T_GEMM_OUT_BF16) ? 1 : 3)) == 0);

@@ -4,9 +4,9 @@
 // That order is the ascending order of the 64-bit word  rank = (~monotone(l) << 32) | index  (unique per token), and "what is kept"
 // is  rank <= cut  (top-k and top-p) together with  z - z_max >= log(min_p).
 // Masses are WHOLE NUMBERS: w_i = round(2^F exp(z_i - z_max)), F = min(50, 62 - ceil(log2 V)), the exponential in double precision;
-// what lies 32 or more below the maximum (e^-32 = 1.3e-14) weighs nothing.  Integer sums do not depend on their order: any split of
-// a row over threads, waves or workgroups, and any order of atomics, gives the same sums, the same cut and the same token, bit for
-// bit.  fp32 sums would not do: over a flat vocabulary of 128 k tokens the borders between tokens lie 8e-6 of the whole apart and
+// what lies 32 or more below the maximum (e^-32 = 1.3e-14) weighs nothing.  Integer sums do not depend on their order: any order of
+// atomics gives the same sums, the same cut and the same token, bit for bit; the draw itself not on the split of the row either (what
+// top_p is a share of does in long rows, by 1e-13: k_sample_hist).  fp32 sums would not do: over a flat vocabulary of 128 k tokens the borders between tokens lie 8e-6 of the whole apart and
 // 6e-8 of rounding moves the answer of one row in a hundred.
 // fp64 multiply-adds run at the rate of unpacked fp32 ones on this chip, and the exponential takes a table entry and a short polynomial.
 //
@@ -450,7 +450,9 @@ template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sa
 // A chunk counts before the row's maximum is known (a pass over the logits less): its bins are whole parts of (l - ref) 64 / T from a
 // reference of its own, so they lie across the row's bins floor(64 (z_max - z)).  A token of chunk bin y -- in the row's units -- belongs to
 // the row's bin y - 1 or y; entered at y - 1 throughout, the running sums bound the true ones from above, and one bin on from below:
-// the cut's bin is one of two.  The masses themselves are exact to 1e-13: bin edge times (count + what the tokens exceed it by).
+// the cut's bin is one of two.  Where a chunk's bins lie on the row's to 1e-9 of a bin (integer logits, say) and its reference is not the
+// row's maximum, the rounding of either side may shift a token on a border by one bin more either way (all of it is below 1e-10 of a bin):
+// then the cut's bin is one of four.  The masses themselves are good to 1e-13: bin edge times (count + what the tokens exceed it by).
 struct ZoneRec {
     u64 best;                 // rank of the row's first token (~0: none)
     u64 whole;                // mass of all tokens
@@ -478,7 +480,8 @@ __device__ __forceinline__ RowWs row_ws(const SampleArgs& a, int b) {
     r.list = (u64*)p;
     return r;
 }
-// the lowest float whose at is below `bound` (or, closed, at most that): from the quotient's float, a step or two up or down
+// the lowest float whose at is below `bound` (or, closed, at most that): from the quotient's float by doubling steps, then halving ones.
+// (Two or three steps as a rule; where the border lies near zero, floats are far closer together than `at` resolves.)
 __device__ __forceinline__ float lowest_float(const Weigh& w, double bound, bool closed) {
     auto in = [&](unsigned o) { const double x = w.at(unmono(o)); return closed ? x <= bound : x < bound; };
     const unsigned least = mono(-3.402823466e+38f), most = mono((float)w.top);
@@ -486,9 +489,16 @@ __device__ __forceinline__ float lowest_float(const Weigh& w, double bound, bool
     if (in(least)) return unmono(least);
     unsigned o = mono((float)fmax(w.top - bound / w.s, -3.402823466e+38));
     o = o > most ? most : o;
-    for (int i = 0; i < 8 && o < most && !in(o); ++i) ++o;
-    for (int i = 0; i < 8 && o > least && in(o - 1); ++i) --o;
-    return unmono(o);
+    unsigned out = least, yes = most, step = 1;            // out does not hold, yes does
+    if (in(o)) {
+        yes = o;
+        while (yes - least > step) { const unsigned n = yes - step; if (!in(n)) { out = n; break; } yes = n; step *= 2; }
+    } else {
+        out = o;
+        while (most - out > step) { const unsigned n = out + step; if (in(n)) { yes = n; break; } out = n; step *= 2; }
+    }
+    while (yes - out > 1) { const unsigned n = out + (yes - out) / 2; if (in(n)) yes = n; else out = n; }
+    return unmono(yes);
 }
 template <bool BF16> __global__ __launch_bounds__(256) void k_sample_hist(SampleArgs a) {
     constexpr int NT = 256, E = Row<BF16>::E, TG = SMP_TILE / E, NQ = TG / NT;
@@ -556,12 +566,13 @@ __global__ __launch_bounds__(512) void k_sample_zone(SampleArgs a) {
     __shared__ double edge[SMP_TILES_MAX];
     __shared__ u64 bin_m[SMP_BINS], first_m;
     __shared__ unsigned bin_c[SMP_BINS], first_c;
-    __shared__ int shift[SMP_TILES_MAX];
+    __shared__ int shift[SMP_TILES_MAX], wide;
     const int b = blockIdx.x, tid = threadIdx.x;
     const Settings st = settings_of(a, b);
     const RowWs ws = row_ws(a, b);
     ZoneRec& rec = *ws.rec;
     exp_tab_begin(tab);
+    if (tid == 0) wide = 0;
     u64 best = tid < a.G ? ws.chunk[tid].best : ~0ull;
     best = block_min<NT>(best, red);
     const Weigh w(&tab, rank_value(best), st, a.frac);
@@ -579,6 +590,7 @@ __global__ __launch_bounds__(512) void k_sample_zone(SampleArgs a) {
         const Chunk c = ws.chunk[tid];
         // the chunk's bin 0 lies at d .. of the row's units (>= 0: the row's largest is no smaller than the chunk's)
         const double d = c.best == ~0ull ? 1e300 : fmax(((double)rank_value(best) - c.ref) * (64.0 / (double)st.T) - c.g_top, 0.0), fl = floor(d);
+        if (c.ref != (double)rank_value(best) && fabs(d - rint(d)) < 1e-9 && fl <= (double)SMP_BINS) wide = 1;
         shift[tid] = fl < (double)SMP_BINS ? (int)fl : SMP_BINS;
         edge[tid] = fl < (double)SMP_BINS ? exp((d - fl) * (-1.0 / 64.0)) : 0.0;
     }
@@ -637,10 +649,11 @@ __global__ __launch_bounds__(512) void k_sample_zone(SampleArgs a) {
         for (int j = 0; j < PER; ++j) { if (cc < (u64)st.k && cc + c[j] >= (u64)st.k) zs[0] = (u64)(tid * PER + j); cc += c[j]; }
         __syncthreads();
         bk = (int)zs[0];
-        // bins in front of bk lie in the top-k; their mass is at least what is entered in front of bk - 1
-        if (bk - 1 >= tid * PER && bk - 1 < (tid + 1) * PER) { u64 mm = mb; for (int j = 0; tid * PER + j < bk - 1; ++j) mm += m[j]; zs[2] = mm; }
+        // bins in front of bk (bk - 1) lie in the top-k; their mass is at least what is entered in front of bk - 1 (bk - 3)
+        const int sure = bk - (wide ? 3 : 1);
+        if (sure >= tid * PER && sure < (tid + 1) * PER) { u64 mm = mb; for (int j = 0; tid * PER + j < sure; ++j) mm += m[j]; zs[2] = mm; }
         __syncthreads();
-        least = bk >= 1 ? zs[2] : 0;
+        least = sure >= 0 ? zs[2] : 0;
     }
     int b0 = bk;
     if (st.use_p) {
@@ -651,9 +664,12 @@ __global__ __launch_bounds__(512) void k_sample_zone(SampleArgs a) {
         __syncthreads();
         if (zs[1] != ~0ull) b0 = min(bk, (int)zs[1]);
     }
-    if (tid == 64 && b0 < SMP_BINS) rec.v_front = lowest_float(w, (double)b0, false);
-    if (tid == 128 && b0 < SMP_BINS) rec.v_zone = lowest_float(w, (double)((cut_k ? bk : b0) + 2), false);
-    if (tid == 0 && b0 < SMP_BINS) { rec.whole = mall; rec.b0 = b0; rec.b1 = (cut_k ? bk : b0) + 1; rec.cut_k = cut_k; rec.cut_p = st.use_p; }
+    if (b0 == SMP_BINS) return;
+    const int b1 = (cut_k ? bk : b0) + 1 + wide;
+    b0 = max(b0 - wide, 0);
+    if (tid == 64) rec.v_front = lowest_float(w, (double)b0, false);
+    if (tid == 128) rec.v_zone = lowest_float(w, (double)(b1 + 1), false);
+    if (tid == 0) { rec.whole = mall; rec.b0 = b0; rec.b1 = b1; rec.cut_k = cut_k; rec.cut_p = st.use_p; }
 }
 
 template <bool BF16> __global__ __launch_bounds__(256, 6) void k_sample_gather(SampleArgs a) {
@@ -829,9 +845,11 @@ template <bool BF16> __global__ __launch_bounds__(512) void k_sample_draw(Sample
                 mm += m[j];
             }
             __syncthreads();
-            const int i = (int)zs[1];
-            const u64 cp = select_rank<NT, true>(in_sub(i), cut, (int)sub_c[i], need - zs[2], w, L, red, to);
-            cut = cp < cut ? cp : cut;
+            if (zs[1] != ~0ull) {                          // (else the zone's tokens weigh nothing: no matter which are kept)
+                const int i = (int)zs[1];
+                const u64 cp = select_rank<NT, true>(in_sub(i), cut, (int)sub_c[i], need - zs[2], w, L, red, to);
+                cut = cp < cut ? cp : cut;
+            }
         }
         each([&](u64 r) {
             if (r <= cut) {

@@ -96,10 +96,11 @@ class DecodingMixin:
             if isinstance(v, torch.Tensor):
                 if v.shape != (B,) or v.device != sm['u'].device:
                     raise ValueError('sample_decode: %s must be a number or a tensor of %d on %s' % (name, B, sm['u'].device))
+                v = v.detach()
                 sm[name].copy_(v.clamp(-1, 2 ** 31 - 1) if name == 'top_k' and v.dtype is torch.int64 else v)
             else:
                 sm[name].fill_(max(-1, min(int(v), 2 ** 31 - 1)) if name == 'top_k' else float(v))
-        sm['u'][:max_len].copy_(u[:max_len])
+        sm['u'][:max_len].copy_(u[:max_len].detach())
         if self._packed != which:
             self.pack(which)
         if not use_graph:

@@ -134,7 +134,7 @@ def _weights(w, cols, bias, out_dtype, relu, index):
 
 
 def matmul_i8(a, w, bias=None, out_dtype=torch.float32, relu=False, out=None):
-    """a . w^T (+ bias) of two Int8Rows: [a.rows, w.rows], the integer sums exact."""
+    """a . w^T (+ bias) of two Int8Rows: [a.rows, w.rows], the integer sums exact.  out (or None): where to, overlapping no input."""
     if not isinstance(a, Int8Rows):
         _bad('a must be Int8Rows')
     q, index = a.q, a.q.get_device()
@@ -148,7 +148,7 @@ def matmul_i8(a, w, bias=None, out_dtype=torch.float32, relu=False, out=None):
 
 
 def linear_i8(x, w, bias=None, out_dtype=torch.float32, relu=False, out=None):
-    """quantize_rows(x) . w^T (+ bias) in one call: x fp32 or bf16 [rows, cols], w Int8Rows."""
+    """quantize_rows(x) . w^T (+ bias) in one call: x fp32 or bf16 [rows, cols], w Int8Rows.  out (or None): where to, overlapping no input."""
     ldx = _matrix(x, 'x', _FLOATS)
     (m, cols), index = x.shape, x.get_device()
     n, b, flags = _weights(w, cols, bias, out_dtype, relu, index)

@@ -331,8 +331,9 @@ int e2t_quant_rows_i8(const void* x, int dtype, long long ldx, int M, int K, int
 /* C[m][n] = sa[m] * sb[n] * sum_k A[m][k] * B[n][k] (+ bias[n]): A int8 [M][lda] (one scale a row = token), B int8 [N][ldb] (one scale a
  * row = output channel), both 16-B aligned with leading dimensions that are multiples of 16 and >= K rounded up to 64; columns
  * from K up to that must be zero in at least one of the two (e2t_quant_rows_i8 writes them so).  The integer sum is exact
- * (K <= E2T_I8_MAX_K), then rounded to fp32 once; scales, bias and the optional ReLU in fp32.  flags: E2T_GEMM_RELU,
- * E2T_GEMM_OUT_BF16 (C bf16 instead of fp32); others are refused. */
+ * (K <= E2T_I8_MAX_K), then rounded to fp32 once and multiplied by sa, then by sb; bias and the optional ReLU in fp32.  flags:
+ * E2T_GEMM_RELU, E2T_GEMM_OUT_BF16 (C bf16 instead of fp32); others are refused.  C overlaps none of the inputs. */
+#define E2T_I8_MAX_ROWS (1 << 30)   /* M, N */
 #define E2T_I8_MAX_K 131071
 #define E2T_I8_MAX_LD 8388608       /* largest lda / ldb: a tile's rows are addressed with 32 bits */
 int e2t_gemm_nt_i8(const int8_t* A, long long lda, const float* sa, const int8_t* B, long long ldb, const float* sb, const float* bias,
@@ -349,8 +350,9 @@ int e2t_linear_i8(const void* x, int dtype, long long ldx, const int8_t* W, long
  * token, by index, at which the kept probabilities' running sum exceeds u times their sum.  temperature <= 0 (or NaN) takes the
  * first token of the ranking.  token[b] = -1 where no logit is above -inf.  logprob[b] (or NULL): the natural logarithm of the
  * token's probability among the kept ones (0 for temperature <= 0, -inf for token -1).
- * The answer does not depend on launch shape, order of sums or other rows: sums are of whole numbers (probability in units of
- * 2^-F of the largest, F = min(50, 62 - ceil(log2 V))).  A settings array, where given, holds one value a row (device memory);
+ * Sums are of whole numbers (probabilities in units of 2^-F of the largest, F = min(50, 62 - ceil(log2 V)), each good to 2e-14 of its
+ * value or half a unit), so the answer does not depend on their order; what lies 32 or more below the largest z weighs nothing.
+ * In rows above 8185 tokens the sum that top_p is a share of is good to 1e-13 only, in a way that depends on B.  A settings array, where given, holds one value a row (device memory);
  * the scalar counts where it is NULL.  ws: device memory of e2t_sample_ws_bytes(B, V), 16-B aligned, needed until the call has run. */
 #define E2T_SAMPLE_MAX_V 1048576
 typedef struct e2t_sample_cfg {

@@ -335,6 +335,45 @@ def test_sample_rows_strided_and_unaligned(S):
             check_sample(S, big[1::2, 3:3 + V], u, top_p=0.9, top_k=30)
 
 
+@pytest.mark.parametrize('T,unit', [(49.0, 49.0), (3.0, 1.0), (7.0, 7.0), (1.0, 0.25), (0.7, 0.7)])
+def test_sample_rows_levels_on_bin_borders(S, T, unit):
+    """Long rows whose logits are a few whole multiples of one number: workgroups that have not seen the largest one count from another
+    level, and every level may lie on a border of the counting."""
+    B, V = 6, 40000
+    g = gen(int(T * 10))
+    level = torch.randint(1, 12, (B, V), generator=g, device='cuda').float()
+    level[:, :V // 2] = level[:, :V // 2].clamp(min=5)
+    level[3:, V // 2:] += 3
+    l = -level * unit
+    l[:, 77] = 0
+    for kw in (dict(top_k=300), dict(top_k=9000), dict(top_k=V - 5), dict(top_k=30000, top_p=0.83), dict(top_p=0.77), dict(top_k=20000, top_p=0.9, min_p=1e-3)):
+        check_sample(S, l, torch.rand(B, generator=g, device='cuda'), temperature=T, **kw)
+
+
+def test_sample_rows_logits_closer_than_their_distances(S):
+    """Most logits so near zero that their distances to the largest are all the same number in double precision: they still rank by value."""
+    B, V = 4, 30000
+    l = torch.randn(B, V, generator=gen(8), device='cuda') * 1e-20
+    l[:, 5] = 1.0
+    l[1, 5] = 2.0
+    for kw in (dict(top_k=50), dict(top_k=20000), dict(top_k=29999), dict(top_k=1)):
+        check_sample(S, l, torch.rand(B, generator=gen(9), device='cuda'), **kw)
+    short = l[:, :6000].contiguous()
+    check_sample(S, short, torch.rand(B, generator=gen(9), device='cuda'), top_k=50)
+
+
+def test_sample_rows_tails_that_weigh_nothing(S):
+    """The longest row: one token and a million whose masses are below half a unit; the nucleus asks for more than the one."""
+    V = 1 << 20
+    l = torch.full((3, V), -29.85, device='cuda')
+    l[:, 31] = 0
+    l[1, 32:] = float('-inf')
+    for kw in (dict(top_p=1 - 2.0 ** -24), dict(top_p=1 - 2.0 ** -24, top_k=500000), dict()):
+        tok, lp = S.sample_rows(l, torch.tensor([0.0, 0.5, 0.9], device='cuda'), **kw)
+        assert tok.tolist() == [31] * 3
+        assert (lp.abs().double().cpu().numpy() <= V * np.exp(-29.85) + lp_bound(0.0, V)).all()      # (at most the whole tail was kept)
+
+
 def test_sample_rows_frequencies(S):
     """Evenly spread u: token counts are the kept probabilities to one count (the inverse of the running sum)."""
     V, n = 50, 4096

@@ -25,7 +25,7 @@ def test_quant_refusals(H):
     f = H.lib.e2t_quant_rows_i8
     x, q, s = 0x10000, 0x20000, 0x30000
     good = [x, 0, 100, 3, 100, q, 128, s, None]
-    for i, v in ((0, None), (0, x + 2), (1, 2), (2, 99), (3, 0), (3, -1), (4, 0), (5, None), (5, q + 8), (6, 127), (6, 120), (6, 112), (7, None)):
+    for i, v in ((0, None), (0, x + 2), (1, 2), (2, 99), (3, 0), (3, -1), (3, (1 << 30) + 1), (4, 0), (5, None), (5, q + 8), (6, 127), (6, 120), (6, 112), (7, None)):
         a = list(good); a[i] = v
         refused(f, *a)
 
@@ -34,7 +34,7 @@ def test_gemm_refusals(H):
     f = H.lib.e2t_gemm_nt_i8
     good = [0x10000, 128, 0x20000, 0x30000, 128, 0x40000, None, 0x50000, 50, 7, 50, 100, 0, None]
     for i, v in ((0, None), (0, 0x10008), (1, 112), (1, 130), (2, None), (3, None), (3, 0x30004), (4, 64), (4, 136), (5, None), (7, None), (7, 0x50002),
-                 (8, 49), (9, 0), (10, 0), (10, -4), (11, 0), (11, 131072), (12, 4), (12, 8), (12, 16), (12, 64)):
+                 (8, 49), (9, 0), (9, (1 << 30) + 1), (10, 0), (10, -4), (11, 0), (11, 131072), (12, 4), (12, 8), (12, 16), (12, 64)):
         a = list(good); a[i] = v
         refused(f, *a)
 
