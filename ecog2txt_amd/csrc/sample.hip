@@ -6,11 +6,11 @@
 // Masses are WHOLE NUMBERS: w_i = round(2^F exp(z_i - z_max)), F = min(50, 62 - ceil(log2 V)), the exponential in double precision;
 // what lies 32 or more below the maximum (e^-32 = 1.3e-14) weighs nothing.  Integer sums do not depend on their order: any order of
 // atomics gives the same sums, the same cut and the same token, bit for bit; the draw itself not on the split of the row either (what
-// top_p is a share of does in long rows, by 1e-13: k_sample_hist).  fp32 sums would not do: over a flat vocabulary of 128 k tokens the borders between tokens lie 8e-6 of the whole apart and
+// top_p is a share of does in long rows, by 6e-12: k_sample_hist).  fp32 sums would not do: over a flat vocabulary of 128 k tokens the borders between tokens lie 8e-6 of the whole apart and
 // 6e-8 of rounding moves the answer of one row in a hundred.
 // fp64 multiply-adds run at the rate of unpacked fp32 ones on this chip, and the exponential takes a table entry and a short polynomial.
 //
-// Finding the cut.  A histogram of 2048 bins of 1/64 in z (count and mass in one 64-bit LDS atomic) says in which bin the k-th token, or
+// Finding the cut.  A histogram of bins of 1/16 or 1/32 in z (counts and masses) says in which bin the k-th token, or
 // p of the mass, lies; only that bin's tokens are ranked among themselves.
 //
 // Rows up to SMP_ROW_MAX tokens: one workgroup a row, the row in registers, one launch (k_sample_row).  Longer rows: four launches, the row
@@ -98,7 +98,7 @@ __device__ __forceinline__ float unmono(unsigned o) { return __uint_as_float((o 
 __device__ __forceinline__ u64 rank_of(float v, int i) { return ((u64)(~mono(v)) << 32) | (unsigned)i; }
 __device__ __forceinline__ float rank_value(u64 c) { return unmono(~(unsigned)(c >> 32)); }
 
-// ---- reductions over a workgroup of NT threads (red: NT / 64 words of LDS; every call starts with a barrier) ---------------------
+// ---- reductions over a workgroup of NT threads (red: NT / 64 words of LDS; a call starts with a barrier, unless red is its own) ----
 // Within a wave by data-parallel moves (shifts by 1, 2, 4, 8 inside a row of 16 lanes, then the rows' last lanes handed on): six dependent
 // steps of a few cycles instead of six trips through LDS.  The whole wave's result is in lane 63.
 template <int CTRL, int ROWS> __device__ __forceinline__ u64 dpp_u64(u64 other, u64 v) {       // `other` where there is no source lane
@@ -125,9 +125,8 @@ __device__ __forceinline__ float wave_max_63(float v) {
     v = dpp_max<0x111, 0xF>(v); v = dpp_max<0x112, 0xF>(v); v = dpp_max<0x114, 0xF>(v); v = dpp_max<0x118, 0xF>(v);
     v = dpp_max<0x142, 0xA>(v); return dpp_max<0x143, 0xC>(v);
 }
-__device__ __forceinline__ u64 shfl_xor_u64(u64 v, int o) {
-    const unsigned lo = __shfl_xor((unsigned)v, o, 64), hi = __shfl_xor((unsigned)(v >> 32), o, 64);
-    return ((u64)hi << 32) | lo;
+__device__ __forceinline__ u64 lane_u64(u64 v, int i) {         // lane i's (i the same in all lanes)
+    return ((u64)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), i) << 32) | (unsigned)__builtin_amdgcn_readlane((int)v, i);
 }
 template <int NT> __device__ __forceinline__ u64 block_min(u64 v, u64* red) {
     v = wave_min_63(v);
@@ -139,10 +138,10 @@ template <int NT> __device__ __forceinline__ u64 block_min(u64 v, u64* red) {
     for (int i = 1; i < NT / 64; ++i) v = red[i] < v ? red[i] : v;
     return v;
 }
-template <int NT> __device__ __forceinline__ float block_max(float v, u64* red, float* wave_top = nullptr) {
+template <int NT, bool OWN = false> __device__ __forceinline__ float block_max(float v, u64* red, float* wave_top = nullptr) {
     v = wave_max_63(v);
     float* r = (float*)red;
-    __syncthreads();
+    if (!OWN) __syncthreads();
     if ((threadIdx.x & 63) == 63) { r[threadIdx.x >> 6] = v; if (wave_top) wave_top[threadIdx.x >> 6] = v; }
     __syncthreads();
     v = r[0];
@@ -151,9 +150,9 @@ template <int NT> __device__ __forceinline__ float block_max(float v, u64* red, 
     return v;
 }
 // exclusive prefix over the threads; total = sum of all
-template <int NT> __device__ __forceinline__ u64 block_scan(u64 v, u64* red, u64& total) {
+template <int NT, bool OWN = false> __device__ __forceinline__ u64 block_scan(u64 v, u64* red, u64& total) {
     const u64 s = wave_scan(v);
-    __syncthreads();
+    if (!OWN) __syncthreads();
     if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = s;
     __syncthreads();
     u64 before = 0, all = 0;
@@ -163,9 +162,9 @@ template <int NT> __device__ __forceinline__ u64 block_scan(u64 v, u64* red, u64
     return before + s - v;
 }
 // two of them with one pair of barriers (red: twice as long)
-template <int NT> __device__ __forceinline__ void block_scan2(u64& v, u64& w, u64* red, u64& total_v, u64& total_w) {
+template <int NT, bool OWN = false> __device__ __forceinline__ void block_scan2(u64& v, u64& w, u64* red, u64& total_v, u64& total_w) {
     const u64 s = wave_scan(v), t = wave_scan(w);
-    __syncthreads();
+    if (!OWN) __syncthreads();
     if ((threadIdx.x & 63) == 63) { red[threadIdx.x >> 6] = s; red[NT / 64 + (threadIdx.x >> 6)] = t; }
     __syncthreads();
     u64 bv = 0, bw = 0, av = 0, aw = 0;
@@ -181,25 +180,47 @@ template <int NT> __device__ __forceinline__ void block_scan2(u64& v, u64& w, u6
 
 // ---- weights ------------------------------------------------------------------------------------------------------------------------
 // 2^F exp(-at / 64), at >= 0: the nearest whole number's from a table in LDS (made as the product of two short ones; what lies 2048
-// or further down weighs nothing), the rest from the polynomial of degree 4 through the Chebyshev nodes of [-1/2, 1/2] (off by at most
-// 1.5e-14 of exp): about 18 instructions a token, and no branch between the tokens of a thread, so that their chains interleave.
-struct ExpTab { double e[SMP_BINS + 1], a[32], b[64]; };
-__device__ __forceinline__ void exp_tab_begin(ExpTab& t) {             // (a barrier between begin and fill, one between fill and use)
-    if (threadIdx.x < 32) t.a[threadIdx.x] = exp(-(double)threadIdx.x);
-    else if (threadIdx.x >= 64 && threadIdx.x < 128) t.b[threadIdx.x - 64] = exp(-(double)(threadIdx.x - 64) / 64.0);
-}
-template <int NT> __device__ __forceinline__ void exp_tab_fill(ExpTab& t, int frac) {
-    const double scale = (double)(1ull << frac);
+// or further down weighs nothing), the rest from a polynomial: about 18 instructions a token, and no branch between the tokens of a thread, so that their chains interleave.
+// exp(-n) and exp(-n / 64), rounded to the nearest: loads that travel with the logits', where exp() itself would take 0.5 us
+__device__ const double smp_exp_a[32] = {
+    0x1.0000000000000p+0, 0x1.78b56362cef38p-2, 0x1.152aaa3bf81ccp-3, 0x1.97db0ccceb0afp-5, 0x1.2c155b8213cf4p-6, 0x1.b993fe00d5376p-8,
+    0x1.44e51f113d4d6p-9, 0x1.de16b9c24a98fp-11, 0x1.5fc21041027adp-12, 0x1.02cf22526545ap-13, 0x1.7cd79b5647c9bp-15, 0x1.18354238f6764p-16,
+    0x1.9c54c3b43bc8bp-18, 0x1.2f6053b981d98p-19, 0x1.be6c6fdb01612p-21, 0x1.4875ca227ec38p-22, 0x1.e355bbaee85cbp-24, 0x1.639e3175a689dp-25,
+    0x1.05a628c699fa1p-26, 0x1.81056ff2c5772p-28, 0x1.1b48655f37267p-29, 0x1.a0db0d0ddb3ecp-31, 0x1.32b48bf117da2p-32, 0x1.c3527e433fab1p-34,
+    0x1.4c1078fe9228ap-35, 0x1.e8a37a45fc32ep-37, 0x1.67852a7007e42p-38, 0x1.0885298767e9ap-39, 0x1.853f01d6d53bap-41, 0x1.1e642baeb84a0p-42,
+    0x1.a56e0c2ac7f75p-44, 0x1.36121e24d3bbap-45};
+__device__ const double smp_exp_b[64] = {
+    0x1.0000000000000p+0, 0x1.f80feabfeefa5p-1, 0x1.f03f56a88b5d8p-1, 0x1.e88dc6afecfc0p-1, 0x1.e0fabfbc702a4p-1, 0x1.d985c89d041a3p-1,
+    0x1.d22e6a0197c03p-1, 0x1.caf42e73a4c7ep-1, 0x1.c3d6a24ed8222p-1, 0x1.bcd553b9d7b62p-1, 0x1.b5efd29f24c26p-1, 0x1.af25b0a61a7b5p-1,
+    0x1.a876812c0877cp-1, 0x1.a1e1d93d687d0p-1, 0x1.9b674f8f2f3d8p-1, 0x1.95067c78379f2p-1, 0x1.8ebef9eac820bp-1, 0x1.8890636e31f54p-1,
+    0x1.827a561889716p-1, 0x1.7c7c70887763cp-1, 0x1.769652df22f7ep-1, 0x1.70c79eba33c07p-1, 0x1.6b0ff72deb89dp-1, 0x1.656f00bf5796ap-1,
+    0x1.5fe4615e98e8fp-1, 0x1.5a6fc061433c8p-1, 0x1.5510c67cd2591p-1, 0x1.4fc71dc135627p-1, 0x1.4a9271936fd09p-1, 0x1.45726ea84fb88p-1,
+    0x1.4066c2ff39127p-1, 0x1.3b6f1ddd05a92p-1, 0x1.368b2fc6f960ap-1, 0x1.31baaa7dca843p-1, 0x1.2cfd40f8bdcaep-1, 0x1.2852a760d5c59p-1,
+    0x1.23ba930c1568bp-1, 0x1.1f34ba78d5666p-1, 0x1.1ac0d5492c0dcp-1, 0x1.165e9c3e67663p-1, 0x1.120dc934993e8p-1, 0x1.0dce171e34e7fp-1,
+    0x1.099f41ffbe580p-1, 0x1.058106eb8a6aap-1, 0x1.017323fd90020p-1, 0x1.faeab0ae9381dp-2, 0x1.f30ec8375038bp-2, 0x1.eb5210d6270b7p-2,
+    0x1.e3b40ebefcd7ep-2, 0x1.dc3448110daaep-2, 0x1.d4d244cf4ea9ep-2, 0x1.cd8d8ed8ee386p-2, 0x1.c665b1e1f1e0dp-2, 0x1.bf5a3b6bf18b7p-2,
+    0x1.b86ababeef8dfp-2, 0x1.b196c0e24d229p-2, 0x1.aadde095dad4bp-2, 0x1.a43fae4b0474ep-2, 0x1.9dbbc01e18268p-2, 0x1.9751adcfa81c1p-2,
+    0x1.910110be06976p-2, 0x1.8ac983dedbc65p-2, 0x1.84aaa3b8d514ep-2, 0x1.7ea40e5d6d8fap-2};
+struct ExpTab { double e[SMP_BINS + 1]; };
+template <int NT> __device__ __forceinline__ void exp_tab_fill(ExpTab& t, int frac) {          // (a barrier before the first use)
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const double b = smp_exp_b[threadIdx.x & 63] * (double)(1ull << frac);
 #pragma unroll
-    for (int n = threadIdx.x; n < SMP_BINS; n += NT) t.e[n] = t.a[n >> 6] * t.b[n & 63] * scale;
+    for (int j = 0; j < SMP_BINS / NT; ++j) t.e[j * NT + threadIdx.x] = smp_exp_a[j * (NT / 64) + wave] * b;
     if (threadIdx.x == 0) t.e[SMP_BINS] = 0.0;
 }
-// 2^38 (exp(f / 64) - 1), 0 <= f < 1, rounded to a whole number, as the low bits of 2^52 + x: the polynomial of degree 4 through the
-// Chebyshev nodes of [0, 1] (off by at most 1.6e-14 of exp)
-__device__ __forceinline__ u64 excess38(double f) {
-    double p = 688.02263742244156;
-    p = __builtin_fma(p, f, 174757.97387092107); p = __builtin_fma(p, f, 33554433.677011274); p = __builtin_fma(p, f, 4294967295.7903161);
+// 2^37 (exp(f / 32) - 1), 0 <= f < 1, rounded to a whole number, as the low bits of 2^52 + x: f times the polynomial of degree 3 through
+// four Chebyshev nodes of [0, 1] (off by at most 0.3)
+__device__ __forceinline__ u64 excess37(double f) {
+    double p = 5530.091479314363;
+    p = __builtin_fma(p, f, 699007.5976518993); p = __builtin_fma(p, f, 67108872.62136903); p = __builtin_fma(p, f, 4294967295.7305384);
     return (u64)__double_as_longlong(__builtin_fma(p, f, 4503599627370496.0)) - 0x4330000000000000ull;
+}
+// exp(-f / 64), -1/2 <= f <= 1/2: the polynomial of degree 4 through the Chebyshev nodes (off by at most 1.5e-14)
+__device__ __forceinline__ double exp64(double f) {
+    double p = 2.483533181583589e-09;
+    p = __builtin_fma(p, f, -6.357853029268959e-07); p = __builtin_fma(p, f, 0.00012207031249960526); p = __builtin_fma(p, f, -0.015624999999848418);
+    return __builtin_fma(p, f, 1.0);
 }
 struct Weigh {
     const ExpTab* tab; double top, s, scale, amax;             // s = 64 / T; amax: min-p as a bound of at
@@ -213,9 +234,7 @@ struct Weigh {
     __device__ __forceinline__ u64 mass(double at) const {
         const double c = fmin(at, (double)SMP_BINS), t = c + 6755399441055744.0;          // (1.5 * 2^52: the low word is the nearest whole number)
         const double f = c - (t - 6755399441055744.0);
-        double p = 2.483533181583589e-09;
-        p = __builtin_fma(p, f, -6.357853029268959e-07); p = __builtin_fma(p, f, 0.00012207031249960526); p = __builtin_fma(p, f, -0.015624999999848418); p = __builtin_fma(p, f, 1.0);
-        return (u64)__double_as_longlong(__builtin_fma(tab->e[(int)(unsigned)__double_as_longlong(t)], p, 4503599627370496.0)) - 0x4330000000000000ull;
+        return (u64)__double_as_longlong(__builtin_fma(tab->e[(int)(unsigned)__double_as_longlong(t)], exp64(f), 4503599627370496.0)) - 0x4330000000000000ull;
     }
     // what counts in the draw
     __device__ __forceinline__ u64 kept(float v, int i, u64 cut) const {
@@ -252,18 +271,20 @@ __device__ __forceinline__ float log_prob(const Weigh& w, double at, u64 all) { 
 // ---- ranking a few tokens among themselves -----------------------------------------------------------------------------------------
 // Of the tokens with rank <= hi that `each` enumerates (at most n, each by exactly one thread): the need-th by count (BY_MASS false; there are
 // as many), or the first at which the running mass reaches need -- the last one where the whole does not; `mass_to`: the mass up to
-// and with it.  While there are more than CAP: a histogram over the eight highest bits in which they differ.
+// and with it.  While there are more than 64: a histogram over the eight highest bits in which they differ.  The rest lie in a list, a lane
+// each, and every wave ranks them for itself against the lanes' values: no barrier behind the one that completes the list (as one
+// list for the workgroup with n^2 comparisons spread over it: 2.2 us a call, most of it barriers and LDS round trips).
+// One call each of either kind in a kernel; L.n is zero at the first.
 template <int NT> struct SelectLds {
-    static constexpr int CAP = NT >= 1024 ? 256 : NT >= 512 ? 180 : 128;       // (n^2 / NT steps to rank n)
     u64 m[256]; unsigned c[256];
-    u64 list[CAP], lm[CAP];
-    unsigned n;
+    u64 list[2][64];
+    unsigned n[2];
     u64 out[3];
 };
 template <int NT, bool BY_MASS, class Each> __device__ __forceinline__ u64 select_rank(Each each, u64 hi, int n, u64 need, const Weigh& w, SelectLds<NT>& L, u64* red,
                                                                                       u64& mass_to) {
     u64 lo = 0, before_m = 0, before_c = 0;
-    while (n > SelectLds<NT>::CAP) {
+    while (__builtin_expect(n > 64, 0)) {
         u64 mn = ~0ull, mx = ~0ull;
         each([&](u64 r) { if (r >= lo && r <= hi) { mn = r < mn ? r : mn; mx = ~r < mx ? ~r : mx; } });
         mn = block_min<NT>(mn, red); mx = ~block_min<NT>(mx, red);
@@ -273,6 +294,7 @@ template <int NT, bool BY_MASS, class Each> __device__ __forceinline__ u64 selec
         __syncthreads();
         const u64 first = mn >> shift;
         each([&](u64 r) {
+            asm volatile("" : "+v"(r));                    // (else the masses of all of the thread's tokens are worked out in front of the loop, 0.5 us for nothing)
             if (r >= lo && r <= hi) { const int d = (int)((r >> shift) - first); atomicAdd(&L.c[d], 1u); atomicAdd(&L.m[d], w.mass(w.at(rank_value(r)))); }
         });
         __syncthreads();
@@ -290,47 +312,43 @@ template <int NT, bool BY_MASS, class Each> __device__ __forceinline__ u64 selec
         n = (int)L.c[d];
         __syncthreads();
     }
-    if (threadIdx.x == 0) L.n = 0;
+    u64* list = L.list[BY_MASS];
+    each([&](u64 r) { if (r >= lo && r <= hi) { const unsigned k = atomicAdd(&L.n[BY_MASS], 1u); if (k < 64) list[k] = r; } });
     __syncthreads();
-    each([&](u64 r) { if (r >= lo && r <= hi) { const unsigned k = atomicAdd(&L.n, 1u); if (k < (unsigned)SelectLds<NT>::CAP) L.list[k] = r; } });
-    __syncthreads();
-    n = (int)L.n;
+    n = __builtin_amdgcn_readfirstlane((int)L.n[BY_MASS]);
     if (n == 0) { mass_to = before_m; return ~0ull; }
-    if ((int)threadIdx.x < n) L.lm[threadIdx.x] = w.mass(w.at(rank_value(L.list[threadIdx.x])));
-    __syncthreads();
-    // g threads (a power of two, within a wave) share the comparisons of one token
-    int g = 1;
-    while (g < 64 && n > 16 * g && n * g * 2 <= NT) g *= 2;
-    const int e = threadIdx.x / g, part = threadIdx.x & (g - 1);
-    u64 c = 0, m = 0, mine = 0, own = 0;
-    if (e < n) {
-        mine = L.list[e]; own = L.lm[e];
-        for (int i = part; i < n; i += g) if (L.list[i] <= mine) { ++c; m += L.lm[i]; }
+    const int lane = threadIdx.x & 63;
+    const u64 r = lane < n ? list[lane] : ~0ull, own = lane < n ? w.mass(w.at(rank_value(r))) : 0;
+    u64 m = before_m;
+    unsigned c = 0;
+    for (int i = 0; i < n; i += 4) {                       // (lanes from n on: rank ~0, mass 0)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const u64 ri = lane_u64(r, i + e), mi = lane_u64(own, i + e);
+            c += ri <= r; m += ri <= r ? mi : 0;
+        }
     }
-    for (int o = 1; o < g; o <<= 1) { c += shfl_xor_u64(c, o); m += shfl_xor_u64(m, o); }
-    if (e < n && part == 0 && c == (u64)n) L.out[2] = m;     // (the last of them: the mass of all)
-    __syncthreads();
-    const u64 most = before_m + L.out[2];
-    if (e < n && part == 0) {
-        const u64 nd = BY_MASS ? (need < most ? need : most) : need;
-        const u64 x = BY_MASS ? before_m + m : before_c + c, b = BY_MASS ? x - own : x - 1;
-        if (b < nd && x >= nd) { L.out[0] = mine; L.out[1] = before_m + m; }
-    }
-    __syncthreads();
-    const u64 r = L.out[0];
-    mass_to = L.out[1];
-    __syncthreads();
-    return r;
+    const int last = __ffsll((unsigned long long)__ballot(lane < n && c == (unsigned)n)) - 1;
+    const u64 most = lane_u64(m, last), nd = BY_MASS && need > most ? most : need;
+    const u64 x = BY_MASS ? m : before_c + c, b = BY_MASS ? x - own : x - 1;
+    const u64 hit = __ballot(lane < n && b < nd && x >= nd);
+    const int at = hit ? __ffsll(hit) - 1 : last;
+    mass_to = lane_u64(m, at);
+    return lane_u64(r, at);
 }
 
 // ---- one workgroup a row ---------------------------------------------------------------------------------------------------------------
+// (The histogram here is of 512 bins of 1/16, counts and masses apart: two bins a thread or one, no conversions, and the masses stay
+// in registers for the draw: 1806 tokens with all four settings in 7.4 us, 256 such rows in 8.6.  It is a chain of dependent steps: load 0.7,
+// maximum 0.3, masses and bins 1.3, each cut 1.5, draw and logarithm 1.4.)
 template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sample_row(SampleArgs a) {
-    constexpr int E = Row<BF16>::E, NG = VPT / E, PER = SMP_BINS / NT;
-    __shared__ u64 red[2 * (NT / 64)];
+    constexpr int E = Row<BF16>::E, NG = VPT / E, NB = 512, PER = NB / NT, NW = NT / 64;
+    __shared__ u64 red[6 * NW];                            // (a place for each reduction)
     __shared__ ExpTab tab;
-    __shared__ u64 hist[SMP_BINS];
+    __shared__ u64 hist_m[NB];
+    __shared__ unsigned hist_c[NB];
     __shared__ SelectLds<NT> L;
-    __shared__ u64 zs[4];
+    __shared__ u64 zs[6];
     const int b = blockIdx.x, tid = threadIdx.x;
     const Row<BF16> row(a, b);
     // thread t holds tokens t * VPT - o .. + VPT - 1
@@ -339,17 +357,17 @@ template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sa
     const int i0 = tid * VPT - row.o;
     const Settings st = settings_of(a, b);
     const float u = a.u[b];
-    exp_tab_begin(tab);
+    exp_tab_fill<NT>(tab, a.frac);
 #pragma unroll
-    for (int j = 0; j < PER; ++j) hist[tid + j * NT] = 0;
-    if (tid == 0) zs[0] = zs[1] = ~0ull;
+    for (int j = 0; j < PER; ++j) { hist_m[tid + j * NT] = 0; hist_c[tid + j * NT] = 0; }
+    if (tid == 0) L.n[0] = L.n[1] = 0;
     float v[VPT];
 #pragma unroll
     for (int q = 0; q < NG; ++q) row.unpack(raw[q], v + q * E);
     float top = v[0];
 #pragma unroll
     for (int j = 1; j < VPT; ++j) top = fmaxf(top, v[j]);
-    top = block_max<NT>(top, red);                         // (its barriers publish the short tables and the empty histogram)
+    top = block_max<NT, true>(top, red);                   // (its barrier publishes the table and the empty histogram)
     if (top == -INFINITY) { if (tid == 0) sample_store(a, b, -1, -INFINITY); return; }
     if (st.greedy) {
         u64 best = ~0ull;
@@ -360,30 +378,26 @@ template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sa
         return;
     }
     const Weigh w(&tab, top, st, a.frac);
-    exp_tab_fill<NT>(tab, a.frac);
-    __syncthreads();
-    u64 cut = ~0ull;
+    u64 tm[VPT];
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) tm[j] = w.mass(w.at(v[j]));
+    float cv = -INFINITY;                                  // kept: logit above cv, or equal and index up to ci
+    int ci = 0x7FFFFFFF;
     if (st.use_k || st.use_p) {
-        // one word a token: 1 << 48 for the count, and 2^38 (exp(rest / 64) - 1) of what it exceeds the bin's lower edge by (16384 tokens: below 2^46)
         short bin[VPT];
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             const double at = w.at(v[j]);
-            const int n = at < (double)SMP_BINS ? (int)at : SMP_BINS;
+            const int n = at < (double)SMP_BINS ? (int)(at * ((double)NB / SMP_BINS)) : NB;
             bin[j] = (short)n;
-            if (n < SMP_BINS) atomicAdd(&hist[n], (1ull << 48) + excess38((double)(n + 1) - at));
+            if (n < NB) { atomicAdd(&hist_c[n], 1u); atomicAdd(&hist_m[n], tm[j]); }
         }
         __syncthreads();
         u64 c[PER], m[PER], cs = 0, ms = 0;
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const u64 h = hist[tid * PER + j];
-            c[j] = h >> 48;
-            m[j] = (u64)(((double)(unsigned)c[j] + (double)(long long)(h & 0xFFFFFFFFFFFFull) * 0x1p-38) * tab.e[tid * PER + j + 1] + 0.5);
-            cs += c[j]; ms += m[j];
-        }
-        u64 call, mall, cb = cs, mb = ms;
-        block_scan2<NT>(cb, mb, red, call, mall);
+        for (int j = 0; j < PER; ++j) { c[j] = hist_c[tid * PER + j]; m[j] = hist_m[tid * PER + j]; cs += c[j]; ms += m[j]; }
+        u64 call, mass, cb = cs, mb = ms;
+        block_scan2<NT, true>(cb, mb, red + NW, call, mass);
         // tokens of one bin, by rank
         auto in_bin = [&](int n) {
             return [&, n](auto f) {
@@ -391,8 +405,7 @@ template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sa
                 for (int j = 0; j < VPT; ++j) if (bin[j] == n) f(rank_of(v[j], i0 + j));
             };
         };
-        u64 mass = mall;
-        int bk = SMP_BINS;
+        u64 cut = ~0ull;
         if (st.use_k && (u64)st.k < call) {
             u64 cc = cb, mm = mb;
 #pragma unroll
@@ -401,42 +414,42 @@ template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sa
                 cc += c[j]; mm += m[j];
             }
             __syncthreads();
-            bk = (int)zs[0];
             const u64 before = zs[2] & 0xFFFFFFFFull, above = zs[3];
             u64 to;
-            cut = select_rank<NT, false>(in_bin(bk), ~0ull, (int)(zs[2] >> 32), (u64)st.k - before, w, L, red, to);
+            cut = select_rank<NT, false>(in_bin((int)zs[0]), ~0ull, (int)(zs[2] >> 32), (u64)st.k - before, w, L, red + 3 * NW, to);
             mass = above + to;
         }
         if (st.use_p) {
-            const u64 need = p_need(st.P, mass);
+            const u64 need = p_need(st.P, mass);           // (at most the mass: a bin holds it)
             u64 mm = mb;
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
-                if (tid * PER + j <= bk && mm < need && mm + m[j] >= need) { zs[1] = (u64)(tid * PER + j); zs[2] = c[j]; zs[3] = mm; }
+                if (mm < need && mm + m[j] >= need) { zs[1] = (u64)(tid * PER + j); zs[4] = c[j]; zs[5] = mm; }
                 mm += m[j];
             }
             __syncthreads();
-            if (zs[1] != ~0ull) {
-                u64 to;
-                const u64 cp = select_rank<NT, true>(in_bin((int)zs[1]), cut, (int)zs[2], need - zs[3], w, L, red, to);
-                cut = cp < cut ? cp : cut;
-            }
+            u64 to;
+            cut = select_rank<NT, true>(in_bin((int)zs[1]), cut, (int)zs[4], need - zs[5], w, L, red + 3 * NW, to);
         }
+        if (cut != ~0ull) { cv = rank_value(cut); ci = (int)(unsigned)cut; }
     }
     // the draw: running sums in the order of the vocabulary
     u64 s = 0;
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) s += w.kept(v[j], i0 + j, cut);
+    for (int j = 0; j < VPT; ++j) {
+        const bool in = v[j] > cv || (v[j] == cv && i0 + j <= ci);
+        tm[j] = in && (!st.use_m || w.at(v[j]) <= w.amax) ? tm[j] : 0;
+        s += tm[j];
+    }
     u64 all;
-    u64 before = block_scan<NT>(s, red, all);
+    u64 before = block_scan<NT, true>(s, red + 5 * NW, all);
     const u64 r = u_times(u, all);
     if (before <= r && r < before + s) {
         int pick = -1; float pv = 0.f;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-            const u64 m = w.kept(v[j], i0 + j, cut);
-            if (pick < 0 && r < before + m) { pick = i0 + j; pv = v[j]; }
-            before += m;
+            if (pick < 0 && r < before + tm[j]) { pick = i0 + j; pv = v[j]; }
+            before += tm[j];
         }
         sample_store(a, b, pick, log_prob(w, w.at(pv), all));
     }
@@ -447,12 +460,13 @@ template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sa
 // k_sample_gather (mass above the cut of every tile that reaches it, and a list of the tokens in the cut's bins), k_sample_draw (the cut, the
 // tile, the token).  Tiles whose maximum lies below the cut are not read again.
 //
-// A chunk counts before the row's maximum is known (a pass over the logits less): its bins are whole parts of (l - ref) 64 / T from a
-// reference of its own, so they lie across the row's bins floor(64 (z_max - z)).  A token of chunk bin y -- in the row's units -- belongs to
+// A chunk counts before the row's maximum is known (a pass over the logits less): its bins are whole parts of (l - ref) 32 / T from a
+// reference of its own, so they lie across the row's bins floor(32 (z_max - z)).  A token of chunk bin y -- in the row's units -- belongs to
 // the row's bin y - 1 or y; entered at y - 1 throughout, the running sums bound the true ones from above, and one bin on from below:
 // the cut's bin is one of two.  Where a chunk's bins lie on the row's to 1e-9 of a bin (integer logits, say) and its reference is not the
 // row's maximum, the rounding of either side may shift a token on a border by one bin more either way (all of it is below 1e-10 of a bin):
-// then the cut's bin is one of four.  The masses themselves are good to 1e-13: bin edge times (count + what the tokens exceed it by).
+// then the cut's bin is one of four.  The masses themselves are good to 6e-12: bin edge times (count + what the tokens exceed it by).
+#define SMP_LBINS 1024
 struct ZoneRec {
     u64 best;                 // rank of the row's first token (~0: none)
     u64 whole;                // mass of all tokens
@@ -462,18 +476,19 @@ struct ZoneRec {
     int b0, b1;               // bins whose tokens are ranked one by one; in front of b0 everything is kept, behind b1 nothing
     int cut_k, cut_p;         // what is to be found in them
     unsigned n;               // tokens in them
+    u64 above, above_c;       // mass and count of the tokens in front of them
 };
-struct Chunk { double ref, g_top; u64 best; };                 // bin 0 holds tokens with floor((l - ref) 64 / T) = g_top
-struct Tile { u64 all, kept; unsigned count, pad; float top[4]; };    // in front of b0: mass, mass that min-p leaves, tokens; largest logit of each quarter (a wave's)
+struct Chunk { double ref, g_top; u64 best; };                 // bin 0 holds tokens with floor((l - ref) 32 / T) = g_top
+struct Tile { u64 kept; float top[4]; };                       // mass in front of b0 that min-p leaves; largest logit of each quarter (a wave's)
 struct RowWs { u64* hist; Chunk* chunk; Tile* tile; ZoneRec* rec; u64* list; };
 static inline __host__ __device__ size_t ws_up(size_t n) { return (n + 15) & ~(size_t)15; }
 static inline __host__ __device__ size_t row_ws_bytes(int G, int tiles) {
-    return (size_t)G * SMP_BINS * 8 + ws_up(G * sizeof(Chunk)) + ws_up(tiles * sizeof(Tile)) + ws_up(sizeof(ZoneRec)) + (size_t)SMP_LIST * 8;
+    return (size_t)G * SMP_LBINS * 8 + ws_up(G * sizeof(Chunk)) + ws_up(tiles * sizeof(Tile)) + ws_up(sizeof(ZoneRec)) + (size_t)SMP_LIST * 8;
 }
 __device__ __forceinline__ RowWs row_ws(const SampleArgs& a, int b) {
     RowWs r;
     char* p = a.ws + (size_t)b * row_ws_bytes(a.G, a.tiles);
-    r.hist = (u64*)p; p += (size_t)a.G * SMP_BINS * 8;
+    r.hist = (u64*)p; p += (size_t)a.G * SMP_LBINS * 8;
     r.chunk = (Chunk*)p; p += ws_up(a.G * sizeof(Chunk));
     r.tile = (Tile*)p; p += ws_up(a.tiles * sizeof(Tile));
     r.rec = (ZoneRec*)p; p += ws_up(sizeof(ZoneRec));
@@ -503,14 +518,14 @@ __device__ __forceinline__ float lowest_float(const Weigh& w, double bound, bool
 template <bool BF16> __global__ __launch_bounds__(256) void k_sample_hist(SampleArgs a) {
     constexpr int NT = 256, E = Row<BF16>::E, TG = SMP_TILE / E, NQ = TG / NT;
     __shared__ u64 red[2 * (NT / 64)];
-    __shared__ u64 ring[SMP_BINS];
+    __shared__ u64 ring[SMP_LBINS];
     const int chunk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
     const Row<BF16> row(a, b);
     const Settings st = settings_of(a, b);
     const bool bins = !st.greedy && (st.use_k || st.use_p);
     const RowWs ws = row_ws(a, b);
     const int t0 = (int)((long long)chunk * a.tiles / a.G), t1 = (int)((long long)(chunk + 1) * a.tiles / a.G);
-    const double sc = 64.0 / (double)st.T;
+    const double sc = 32.0 / (double)st.T;
     double ref = 0.0, g_top = -INFINITY;                   // bin 0 of the ring, at place `head`; lower bins lie in front of it
     int head = 0;
     float bv = -INFINITY; int bi = 0;
@@ -534,82 +549,81 @@ template <bool BF16> __global__ __launch_bounds__(256) void k_sample_hist(Sample
         mx = block_max<NT>(mx, red, ws.tile[t].top);
         if (!bins || mx == -INFINITY) continue;
         const double g = floor(((double)mx - ref) * sc);
-        if (!(g - g_top < (double)SMP_BINS)) {             // the first tokens, or all before lie below the window: start anew from here
+        if (!(g - g_top < (double)SMP_LBINS)) {             // the first tokens, or all before lie below the window: start anew from here
             ref = (double)mx; g_top = 0.0; head = 0;
-            for (int i = tid; i < SMP_BINS; i += NT) ring[i] = 0;
+            for (int i = tid; i < SMP_LBINS; i += NT) ring[i] = 0;
             __syncthreads();
         } else if (g > g_top) {                            // the window moves up: its new bins start empty
             const int nz = (int)(g - g_top);
-            for (int i = tid; i < nz; i += NT) ring[(head + 1 + i) & (SMP_BINS - 1)] = 0;
-            head = (head + nz) & (SMP_BINS - 1);
+            for (int i = tid; i < nz; i += NT) ring[(head + 1 + i) & (SMP_LBINS - 1)] = 0;
+            head = (head + nz) & (SMP_LBINS - 1);
             g_top = g;
             __syncthreads();
         }
-        // one word a token: 1 << 48 for the count, and 2^38 (exp(rest / 64) - 1) of what it exceeds the bin's edge by (49152 tokens: below 2^48)
+        // one word a token: 1 << 48 for the count, and 2^37 (exp(rest / 32) - 1) of what it exceeds the bin's edge by (49152 tokens: below 2^48)
 #pragma unroll
         for (int j = 0; j < NQ * E; ++j) {
             const double x = ((double)v[j] - ref) * sc, fl = floor(x), rel = g_top - fl;
-            if (rel < (double)SMP_BINS) atomicAdd(&ring[(head - (int)rel) & (SMP_BINS - 1)], (1ull << 48) + excess38(x - fl));
+            if (rel < (double)SMP_LBINS) atomicAdd(&ring[(head - (int)rel) & (SMP_LBINS - 1)], (1ull << 48) + excess37(x - fl));
         }
     }
     const u64 best = block_min<NT>(bv == -INFINITY ? ~0ull : rank_of(bv, bi), red);
     if (tid == 0) { ws.chunk[chunk].best = best; ws.chunk[chunk].ref = ref; ws.chunk[chunk].g_top = g_top; }
-    if (bins && best != ~0ull) for (int i = tid; i < SMP_BINS; i += NT) ws.hist[(size_t)chunk * SMP_BINS + i] = ring[(head - i) & (SMP_BINS - 1)];
+    if (bins && best != ~0ull) for (int i = tid; i < SMP_LBINS; i += NT) ws.hist[(size_t)chunk * SMP_LBINS + i] = ring[(head - i) & (SMP_LBINS - 1)];
 }
 
 #define SMP_TILES_MAX (E2T_SAMPLE_MAX_V / SMP_TILE + 1)
 __global__ __launch_bounds__(512) void k_sample_zone(SampleArgs a) {
-    constexpr int NT = 512, PER = SMP_BINS / NT;
-    __shared__ u64 red[2 * (NT / 64)];
+    constexpr int NT = 512, PER = SMP_LBINS / NT;
+    __shared__ u64 red[3 * (NT / 64)];
     __shared__ ExpTab tab;
     __shared__ u64 zs[4];
     __shared__ double edge[SMP_TILES_MAX];
-    __shared__ u64 bin_m[SMP_BINS], first_m;
-    __shared__ unsigned bin_c[SMP_BINS], first_c;
+    __shared__ u64 bin_m[SMP_LBINS], first_m;
+    __shared__ unsigned bin_c[SMP_LBINS], first_c;
     __shared__ int shift[SMP_TILES_MAX], wide;
     const int b = blockIdx.x, tid = threadIdx.x;
-    const Settings st = settings_of(a, b);
     const RowWs ws = row_ws(a, b);
+    const Chunk mine = ws.chunk[min(tid, a.G - 1)];
+    const Settings st = settings_of(a, b);
     ZoneRec& rec = *ws.rec;
-    exp_tab_begin(tab);
-    if (tid == 0) wide = 0;
-    u64 best = tid < a.G ? ws.chunk[tid].best : ~0ull;
-    best = block_min<NT>(best, red);
-    const Weigh w(&tab, rank_value(best), st, a.frac);
-    if (tid == 0) {
-        rec.best = best; rec.n = 0; rec.whole = 0; rec.cut_k = rec.cut_p = 0; rec.b0 = SMP_BINS + 1; rec.b1 = SMP_BINS;
-        rec.top = w.top; rec.s = w.s; rec.amax = w.amax; rec.P = st.P; rec.k = st.k; rec.greedy = st.greedy;
-        if (best != ~0ull && !st.greedy) {
-            rec.v_front = rec.v_zone = lowest_float(w, (double)SMP_BINS, false);
-            rec.v_min = w.amax < (double)SMP_BINS ? lowest_float(w, w.amax, true) : rec.v_front;
-        }
-    }
-    if (best == ~0ull || st.greedy || (!st.use_k && !st.use_p)) return;
     exp_tab_fill<NT>(tab, a.frac);
-    if (tid < a.G) {
-        const Chunk c = ws.chunk[tid];
-        // the chunk's bin 0 lies at d .. of the row's units (>= 0: the row's largest is no smaller than the chunk's)
-        const double d = c.best == ~0ull ? 1e300 : fmax(((double)rank_value(best) - c.ref) * (64.0 / (double)st.T) - c.g_top, 0.0), fl = floor(d);
-        if (c.ref != (double)rank_value(best) && fabs(d - rint(d)) < 1e-9 && fl <= (double)SMP_BINS) wide = 1;
-        shift[tid] = fl < (double)SMP_BINS ? (int)fl : SMP_BINS;
-        edge[tid] = fl < (double)SMP_BINS ? exp((d - fl) * (-1.0 / 64.0)) : 0.0;
+    if (tid == 0) { wide = 0; zs[0] = zs[1] = ~0ull; first_m = 0; first_c = 0; }
+    const u64 best = block_min<NT>(mine.best, red);        // (the last chunk's many times)
+    const Weigh w(&tab, rank_value(best), st, a.frac);
+    const bool none = best == ~0ull, cuts = !none && !st.greedy && (st.use_k || st.use_p);
+    if (tid == 0) {
+        rec.best = best; rec.n = 0; rec.above = rec.above_c = 0; rec.whole = 0; rec.cut_k = rec.cut_p = 0; rec.b0 = SMP_LBINS + 1; rec.b1 = SMP_LBINS;
+        rec.top = w.top; rec.s = w.s; rec.amax = w.amax; rec.P = st.P; rec.k = st.k; rec.greedy = st.greedy;
     }
-    if (tid == 0) { zs[0] = zs[1] = ~0ull; first_m = 0; first_c = 0; }
+    if (tid == 192 && !none && !st.greedy) rec.v_min = w.amax < (double)SMP_BINS ? lowest_float(w, w.amax, true) : lowest_float(w, (double)SMP_BINS, false);
+    if (!cuts) {
+        if (tid == 64 && !none && !st.greedy) rec.v_front = rec.v_zone = lowest_float(w, (double)SMP_BINS, false);
+        return;
+    }
+    if (tid < a.G) {
+        // the chunk's bin 0 lies at d .. of the row's units (>= 0: the row's largest is no smaller than the chunk's)
+        const double d = mine.best == ~0ull ? 1e300 : fmax(((double)rank_value(best) - mine.ref) * (32.0 / (double)st.T) - mine.g_top, 0.0), fl = floor(d);
+        if (mine.ref != (double)rank_value(best) && fabs(d - rint(d)) < 1e-9 && fl <= (double)SMP_LBINS) wide = 1;
+        shift[tid] = fl < (double)SMP_LBINS ? (int)fl : SMP_LBINS;
+        const double g = 2.0 * (d - fl), n = rint(g);      // (0, 1 or 2)
+        edge[tid] = fl < (double)SMP_LBINS ? exp64(g - n) * smp_exp_b[(int)n] : 0.0;
+    }
     __syncthreads();
     // bin x: the chunks' bins that cover the row's bins x and x + 1, and in front the one that covers bin 0 alone
     auto value = [](u64 w) {                               // count + excess of a word
-        return __builtin_fma((double)(unsigned)((w >> 32) & 0xFFFFu), 0x1p-6, __builtin_fma((double)(unsigned)w, 0x1p-38, (double)(unsigned)(w >> 48)));
+        return __builtin_fma((double)(unsigned)((w >> 32) & 0xFFFFu), 0x1p-5, __builtin_fma((double)(unsigned)w, 0x1p-37, (double)(unsigned)(w >> 48)));
     };
     unsigned cn[PER] = {};
     double ms0[PER] = {};
-    constexpr int UN = 4;
-    for (int k0 = 0; k0 < a.G; k0 += UN) {                 // (loads of four chunks together)
+    constexpr int UN = 8;
+    for (int k0 = 0; k0 < a.G; k0 += UN) {                 // (loads of eight chunks together)
         u64 w[UN][PER];
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
             const int k = min(k0 + u, a.G - 1);
 #pragma unroll
-            for (int j = 0; j < PER; ++j) w[u][j] = ws.hist[(size_t)k * SMP_BINS + min(max(j * NT + tid + 1 - shift[k], 0), SMP_BINS - 1)];
+            for (int j = 0; j < PER; ++j) w[u][j] = ws.hist[(size_t)k * SMP_LBINS + min(max(j * NT + tid + 1 - shift[k], 0), SMP_LBINS - 1)];
         }
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
@@ -617,19 +631,19 @@ __global__ __launch_bounds__(512) void k_sample_zone(SampleArgs a) {
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
                 const int x = j * NT + tid, r = x + 1 - shift[k];
-                const bool on = k0 + u < a.G && r >= 0 && x + 1 < SMP_BINS;
+                const bool on = k0 + u < a.G && r >= 0 && x + 1 < SMP_LBINS;
                 cn[j] += on ? (unsigned)(w[u][j] >> 48) : 0;
                 ms0[j] = __builtin_fma(value(w[u][j]), on ? edge[k] : 0.0, ms0[j]);
             }
         }
     }
     if (tid < a.G && shift[tid] == 0) {
-        const u64 w = ws.hist[(size_t)tid * SMP_BINS];
+        const u64 w = ws.hist[(size_t)tid * SMP_LBINS];
         atomicAdd(&first_c, (unsigned)(w >> 48));
         atomicAdd(&first_m, (u64)(value(w) * edge[tid] * tab.e[0] + 0.5));
     }
 #pragma unroll
-    for (int j = 0; j < PER; ++j) { bin_c[j * NT + tid] = cn[j]; bin_m[j * NT + tid] = (u64)(ms0[j] * tab.e[j * NT + tid + 1] + 0.5); }
+    for (int j = 0; j < PER; ++j) { bin_c[j * NT + tid] = cn[j]; bin_m[j * NT + tid] = (u64)(ms0[j] * tab.e[2 * (j * NT + tid + 1)] + 0.5); }
     __syncthreads();
     u64 c[PER], m[PER], cs = 0, ms = 0;
 #pragma unroll
@@ -639,8 +653,8 @@ __global__ __launch_bounds__(512) void k_sample_zone(SampleArgs a) {
         cs += c[j]; ms += m[j];
     }
     u64 call, mall, cb = cs, mb = ms;
-    block_scan2<NT>(cb, mb, red, call, mall);
-    int bk = SMP_BINS;
+    block_scan2<NT, true>(cb, mb, red + NT / 64, call, mall);
+    int bk = SMP_LBINS;
     u64 least = mall;                                      // the top-k's mass is at least this
     const bool cut_k = st.use_k && (u64)st.k < call;
     if (cut_k) {
@@ -651,9 +665,11 @@ __global__ __launch_bounds__(512) void k_sample_zone(SampleArgs a) {
         bk = (int)zs[0];
         // bins in front of bk (bk - 1) lie in the top-k; their mass is at least what is entered in front of bk - 1 (bk - 3)
         const int sure = bk - (wide ? 3 : 1);
-        if (sure >= tid * PER && sure < (tid + 1) * PER) { u64 mm = mb; for (int j = 0; tid * PER + j < sure; ++j) mm += m[j]; zs[2] = mm; }
-        __syncthreads();
-        least = sure >= 0 ? zs[2] : 0;
+        if (st.use_p && sure >= 0) {
+            if (sure / PER == tid) { u64 mm = mb; for (int j = 0; j < PER; ++j) mm += j < sure % PER ? m[j] : 0; zs[2] = mm; }
+            __syncthreads();
+        }
+        least = st.use_p && sure >= 0 ? zs[2] : 0;
     }
     int b0 = bk;
     if (st.use_p) {
@@ -664,12 +680,12 @@ __global__ __launch_bounds__(512) void k_sample_zone(SampleArgs a) {
         __syncthreads();
         if (zs[1] != ~0ull) b0 = min(bk, (int)zs[1]);
     }
-    if (b0 == SMP_BINS) return;
+    const bool found = b0 < SMP_LBINS;                     // (not where top-k keeps every token that weighs something)
     const int b1 = (cut_k ? bk : b0) + 1 + wide;
     b0 = max(b0 - wide, 0);
-    if (tid == 64) rec.v_front = lowest_float(w, (double)b0, false);
-    if (tid == 128) rec.v_zone = lowest_float(w, (double)(b1 + 1), false);
-    if (tid == 0) { rec.whole = mall; rec.b0 = b0; rec.b1 = b1; rec.cut_k = cut_k; rec.cut_p = st.use_p; }
+    if (tid == 64) rec.v_front = lowest_float(w, found ? 2.0 * b0 : (double)SMP_BINS, false);
+    if (tid == 128) rec.v_zone = lowest_float(w, found ? 2.0 * (b1 + 1) : (double)SMP_BINS, false);
+    if (tid == 0 && found) { rec.whole = mall; rec.b0 = b0; rec.b1 = b1; rec.cut_k = cut_k; rec.cut_p = st.use_p; }
 }
 
 template <bool BF16> __global__ __launch_bounds__(256, 6) void k_sample_gather(SampleArgs a) {
@@ -686,13 +702,11 @@ template <bool BF16> __global__ __launch_bounds__(256, 6) void k_sample_gather(S
     const Row<BF16> row(a, b);
     const Weigh w(&tab, rec.top, rec.s, rec.amax, a.frac);
     const float v_front = rec.v_front, v_zone = rec.v_zone, v_min = rec.v_min;
-    if (!(mx >= v_zone)) { if (tid == 0) { tile.all = tile.kept = 0; tile.count = 0; } return; }
+    if (!(mx >= v_zone)) { if (tid == 0) tile.kept = 0; return; }
     const int place = (tid >> 6) * (TG / 4) + (tid & 63);
     const bool some = tile.top[tid >> 6] >= v_zone;        // (of this wave's quarter)
     uint4 raw[NQ];
     if (some) row.load(t * TG + place, 64, raw);
-    exp_tab_begin(tab);
-    __syncthreads();
     exp_tab_fill<NT>(tab, a.frac);
     __syncthreads();
     u64 s = 0, sk = 0, cnt = 0;                            // cnt: tokens in front of the zone, and 2^32 for each in it
@@ -739,7 +753,10 @@ template <bool BF16> __global__ __launch_bounds__(256, 6) void k_sample_gather(S
         const int i = (t * TG + place + (j / E) * 64) * E - row.o + j % E;
         if (k < SMP_LIST) ws.list[k] = rank_of(row.at(i), i);
     }
-    if (tid == 0) { tile.all = all; tile.kept = kept; tile.count = (unsigned)count; }
+    if (tid == 0) {
+        tile.kept = kept;
+        if (cuts && (unsigned)count) { atomicAdd(&rec.above, all); atomicAdd(&rec.above_c, (u64)(unsigned)count); }
+    }
 }
 
 // The tokens of the zone once more by finer bins, SMP_SUB over its width, counted and weighed in one go: one of these holds the k-th token
@@ -747,7 +764,7 @@ template <bool BF16> __global__ __launch_bounds__(256, 6) void k_sample_gather(S
 #define SMP_SUB 1024
 template <bool BF16> __global__ __launch_bounds__(512) void k_sample_draw(SampleArgs a) {
     constexpr int NT = 512, E = Row<BF16>::E, NG = SMP_TILE / NT / E, PER = SMP_SUB / NT, KEEP = 4;
-    __shared__ u64 red[2 * (NT / 64)];
+    __shared__ u64 red[7 * (NT / 64)];                     // (a place for each reduction)
     __shared__ ExpTab tab;
     __shared__ SelectLds<NT> L;
     __shared__ u64 tsum[SMP_TILES_MAX];
@@ -758,28 +775,26 @@ template <bool BF16> __global__ __launch_bounds__(512) void k_sample_draw(Sample
     const RowWs ws = row_ws(a, b);
     const ZoneRec rec = *ws.rec;
     const float u = a.u[b];
-    const Tile tile = ws.tile[min(tid, a.tiles - 1)];
+    const u64 tile_kept = ws.tile[min(tid, a.tiles - 1)].kept;
+    u64 mine[KEEP], mass_of[KEEP] = {};                    // this thread's part of the list (on its way before it is known how long it is)
+#pragma unroll
+    for (int k = 0; k < KEEP; ++k) mine[k] = ws.list[tid + k * NT];
     if (rec.best == ~0ull) { if (tid == 0) sample_store(a, b, -1, -INFINITY); return; }
     if (rec.greedy) { if (tid == 0) sample_store(a, b, (int)(unsigned)rec.best, 0.0f); return; }
     const bool cuts = rec.cut_k || rec.cut_p, in_list = rec.n <= SMP_LIST;
-    u64 mine[KEEP];                                        // this thread's part of the list
 #pragma unroll
-    for (int k = 0; k < KEEP; ++k) mine[k] = cuts && in_list && tid + k * NT < (int)rec.n ? ws.list[tid + k * NT] : ~0ull;
+    for (int k = 0; k < KEEP; ++k) if (!cuts || !in_list || tid + k * NT >= (int)rec.n) mine[k] = ~0ull;
     const Row<BF16> row(a, b);
-    exp_tab_begin(tab);
-    __syncthreads();
     exp_tab_fill<NT>(tab, a.frac);
+    if (tid == 0) L.n[0] = L.n[1] = 0;
     const Weigh w(&tab, rec.top, rec.s, rec.amax, a.frac);
-    if (tid < a.tiles) tsum[tid] = tile.kept;
+    if (tid < a.tiles) tsum[tid] = tile_kept;
+    if (cuts) for (int i = tid; i < SMP_SUB; i += NT) { sub_m[i] = 0; sub_c[i] = 0; }
+    if (tid == 0) zs[0] = zs[1] = ~0ull;
     __syncthreads();
     u64 cut = ~0ull;
     if (cuts) {
-        for (int i = tid; i < SMP_SUB; i += NT) { sub_m[i] = 0; sub_c[i] = 0; }
-        if (tid == 0) zs[0] = zs[1] = ~0ull;
-        // counts and masses of all tiles in front of the zone
-        u64 above, above_c;
-        u64 ta = tid < a.tiles ? tile.all : 0, tc = tid < a.tiles ? (u64)tile.count : 0;
-        block_scan2<NT>(ta, tc, red, above, above_c);
+        const u64 above = rec.above, above_c = rec.above_c;
         // the tokens of the zone: from the list, or, where they are more than it holds (a flat row), from the row itself
         auto each = [&](auto f) {
             if (in_list) {
@@ -799,8 +814,8 @@ template <bool BF16> __global__ __launch_bounds__(512) void k_sample_draw(Sample
                 }
             }
         };
-        const double fine = (double)SMP_SUB / (double)(rec.b1 + 1 - rec.b0);
-        auto sub_of = [&](u64 r) { return min((int)((w.at(rank_value(r)) - (double)rec.b0) * fine), SMP_SUB - 1); };
+        const double fine = 0.5 * SMP_SUB / (double)(rec.b1 + 1 - rec.b0);
+        auto sub_of = [&](u64 r) { return min((int)((w.at(rank_value(r)) - 2.0 * rec.b0) * fine), SMP_SUB - 1); };
         int my_sub[KEEP];
 #pragma unroll
         for (int k = 0; k < KEEP; ++k) my_sub[k] = mine[k] != ~0ull ? sub_of(mine[k]) : -1;
@@ -812,13 +827,17 @@ template <bool BF16> __global__ __launch_bounds__(512) void k_sample_draw(Sample
                 } else each([&](u64 r) { if (sub_of(r) == i) f(r); });
             };
         };
-        each([&](u64 r) { const int i = sub_of(r); atomicAdd(&sub_c[i], 1u); atomicAdd(&sub_m[i], w.mass(w.at(rank_value(r)))); });
+        auto count_in = [&](int i, u64 m) { atomicAdd(&sub_c[i], 1u); atomicAdd(&sub_m[i], m); };
+        if (rec.n <= KEEP * NT) {
+#pragma unroll
+            for (int k = 0; k < KEEP; ++k) if (my_sub[k] >= 0) { mass_of[k] = w.mass(w.at(rank_value(mine[k]))); count_in(my_sub[k], mass_of[k]); }
+        } else each([&](u64 r) { count_in(sub_of(r), w.mass(w.at(rank_value(r)))); });
         __syncthreads();
         u64 c[PER], m[PER], cs = 0, ms = 0, x;
 #pragma unroll
         for (int j = 0; j < PER; ++j) { c[j] = sub_c[tid * PER + j]; m[j] = sub_m[tid * PER + j]; cs += c[j]; ms += m[j]; }
         u64 cb = cs, mb = ms, xc;
-        block_scan2<NT>(cb, mb, red, xc, x);
+        block_scan2<NT, true>(cb, mb, red, xc, x);
         cb += above_c; mb += above;
         u64 to, mass = rec.whole;
         if (rec.cut_k) {
@@ -831,7 +850,7 @@ template <bool BF16> __global__ __launch_bounds__(512) void k_sample_draw(Sample
             __syncthreads();
             const int i = (int)zs[0];
             const u64 cf = zs[2], mf = zs[3];
-            cut = select_rank<NT, false>(in_sub(i), ~0ull, (int)sub_c[i], (u64)rec.k - cf, w, L, red, to);
+            cut = select_rank<NT, false>(in_sub(i), ~0ull, (int)sub_c[i], (u64)rec.k - cf, w, L, red + 2 * (NT / 64), to);
             mass = mf + to;
         }
         if (rec.cut_p) {
@@ -847,21 +866,20 @@ template <bool BF16> __global__ __launch_bounds__(512) void k_sample_draw(Sample
             __syncthreads();
             if (zs[1] != ~0ull) {                          // (else the zone's tokens weigh nothing: no matter which are kept)
                 const int i = (int)zs[1];
-                const u64 cp = select_rank<NT, true>(in_sub(i), cut, (int)sub_c[i], need - zs[2], w, L, red, to);
+                const u64 cp = select_rank<NT, true>(in_sub(i), cut, (int)sub_c[i], need - zs[2], w, L, red + 2 * (NT / 64), to);
                 cut = cp < cut ? cp : cut;
             }
         }
-        each([&](u64 r) {
-            if (r <= cut) {
-                const double at = w.at(rank_value(r));
-                if (at <= w.amax) atomicAdd(&tsum[((int)(unsigned)r + row.o) / SMP_TILE], w.mass(at));
-            }
-        });
+        auto keep = [&](u64 r, u64 m) { if (r <= cut && w.at(rank_value(r)) <= w.amax) atomicAdd(&tsum[((int)(unsigned)r + row.o) / SMP_TILE], m); };
+        if (rec.n <= KEEP * NT) {
+#pragma unroll
+            for (int k = 0; k < KEEP; ++k) if (my_sub[k] >= 0) keep(mine[k], mass_of[k]);
+        } else each([&](u64 r) { keep(r, w.mass(w.at(rank_value(r)))); });
     }
     __syncthreads();
     const u64 s = tid < a.tiles ? tsum[tid] : 0;
     u64 all;
-    const u64 before = block_scan<NT>(s, red, all);
+    const u64 before = block_scan<NT, true>(s, red + 5 * (NT / 64), all);
     const u64 r = u_times(u, all);
     if (before <= r && r < before + s) { zs[0] = (u64)tid; zs[1] = before; }
     __syncthreads();
@@ -878,7 +896,7 @@ template <bool BF16> __global__ __launch_bounds__(512) void k_sample_draw(Sample
 #pragma unroll
     for (int e = 0; e < NG * E; ++e) ms += w.kept(v[e], i0 + e, cut);
     u64 x;
-    u64 at = in_front + block_scan<NT>(ms, red, x);
+    u64 at = in_front + block_scan<NT, true>(ms, red + 6 * (NT / 64), x);
     if (at <= r && r < at + ms) {
         int pick = -1; float pv = 0.f;
 #pragma unroll
