@@ -6,6 +6,7 @@
 #include "common.h"
 #include "ecog2txt_hip.h"
 #include <atomic>
+#include <type_traits>
 #include <math.h>
 
 #define ST ((hipStream_t)stream)
@@ -91,7 +92,7 @@ struct I8Args {
     const int8_t* A; const int8_t* B; const float* sa; const float* sb; const float* bias; void* C;
     long long lda, ldb, ldc;
     int M, N, S;                  // S: 64-byte k-blocks
-    int relu, out_bf16, vec;      // vec: bytes (16, 8, 4 or an element) that one store may move: every row of the output starts on such a boundary
+    int relu, out_bf16, vec;      // vec: every row of the output starts on a boundary of 16, 8 or 4 bytes (0: of less)
     int full;                     // tiles of the launch that are whole; the workgroups behind them own quarters of one (k_gemm_i8_tile)
     const void* x; long long ldx; int K, xvec, xbf16;     // activations to quantise in the kernel (fused form)
 };
@@ -232,21 +233,28 @@ __device__ __forceinline__ void i8_tile(const I8Args& p, int m0, int n0) {
         char* c = (char*)p.C + ((size_t)mt * p.ldc + n0 + wn) * es;
         const size_t cs = (size_t)p.ldc * es;
         const int nb = ncols * es;                         // bytes of a row
-        if (p.vec == 16 && ncols == CW) {
-            const int ch = CW * es / 16, rpi = 64 / ch;    // 16-B chunks of a row, rows per instruction
-            const int r0 = lane / ch, k = lane - r0 * ch;
-            for (int r = r0; r < nrows; r += rpi) *(uint4*)(c + r * cs + k * 16) = *(const uint4*)(ob + r * RB + k * 16);
-        } else if (p.vec >= 8 && ncols == CW) {
-            constexpr int CH2 = CW / 4;                    // 8-B chunks of a bf16 row; twice as many of fp32
-            const int ch = CH2 * (es >> 1), rpi = 64 / ch;
-            const int r0 = lane / ch, k = lane - r0 * ch;
-            for (int r = r0; r < nrows; r += rpi) *(uint2*)(c + r * cs + k * 8) = *(const uint2*)(ob + r * RB + k * 8);
-        } else if (p.vec >= 4 && (nb & 3) == 0) {
-            for (int r = 0; r < nrows; ++r)
-                for (int k = lane * 4; k < nb; k += 256) *(unsigned*)(c + r * cs + k) = *(const unsigned*)(ob + r * RB + k);
+        // as many bytes a lane as the rows' alignment allows; all of the wave's rows are read before the first is stored (with a loop in which each
+        // store waited for its own LDS read, 7398 x 4337 x 812 took 70 us by elements, so 53; in whole 16 bytes (4336) 49, so 45)
+        auto put = [&](auto type, auto places) {
+            using T = decltype(type);
+            constexpr int PER = decltype(places)::value, RPI = 64 / PER, N = 16 / RPI;          // places of a row, rows an instruction
+            const int rr = lane / PER, k = (lane % PER) * (int)sizeof(T);
+            T v[N];
+#pragma unroll
+            for (int n = 0; n < N; ++n) v[n] = *(const T*)(ob + (rr + n * RPI) * RB + k);
+#pragma unroll
+            for (int n = 0; n < N; ++n) if (rr + n * RPI < nrows && k < nb) *(T*)(c + (rr + n * RPI) * cs + k) = v[n];
+        };
+        const int vec = ncols == CW ? p.vec : p.vec >= 4 && (nb & 3) == 0 ? 4 : 0;
+        if (es == 4) {
+            if (vec == 16) put(make_uint4(0, 0, 0, 0), std::integral_constant<int, CW / 4>{});
+            else if (vec == 8) put(make_uint2(0, 0), std::integral_constant<int, CW / 2>{});
+            else put(0u, std::integral_constant<int, CW>{});
         } else {
-            for (int r = 0; r < nrows; ++r)
-                for (int k = lane * 2; k < nb; k += 128) *(bf16_t*)(c + r * cs + k) = *(const bf16_t*)(ob + r * RB + k);
+            if (vec == 16) put(make_uint4(0, 0, 0, 0), std::integral_constant<int, CW / 8>{});
+            else if (vec == 8) put(make_uint2(0, 0), std::integral_constant<int, CW / 4>{});
+            else if (vec == 4) put(0u, std::integral_constant<int, CW / 2>{});
+            else put((unsigned short)0, std::integral_constant<int, CW>{});
         }
     }
 }
@@ -290,9 +298,11 @@ __global__ __launch_bounds__(64 * WM * WN * KS, WM * WN * KS * WGS / 4) void k_g
 // loads run at 36 GB/s a CU whatever the shape -- in MFMA order neighbouring lanes belong to different rows, four cache lines a
 // quad of lanes --, through LDS a quad reads one 64-byte line.  The waves' partial sums meet in LDS (integer adds: their order
 // does not matter).
-// FUSED: the activations are x (fp32 / bf16), quantised by every workgroup for itself into LDS while its first weights are on their way.
+// FUSED: the activations are x (fp32 / bf16, up to 8 rows), quantised by every workgroup for itself into LDS while its first weights are on
+// their way.
 template <int MT, int NTL, int NWV, int D, int FUSED /* 0 no, 1 fp32, 2 bf16 */>
 __global__ __launch_bounds__(64 * NWV) void k_gemm_i8_rows(I8Args p) {
+    static_assert(!FUSED || NWV == 8, "a wave for each of the rows");
     constexpr int NT = 64 * NWV, MR = MT * 16, NC = NTL * 16, NP = (FUSED ? 0 : MT) + NTL, RING = D * NP * 1024;
     __shared__ int part[MR * NC];
     __shared__ float red[NWV], sxs[FUSED ? MR : 1];
@@ -324,34 +334,29 @@ __global__ __launch_bounds__(64 * NWV) void k_gemm_i8_rows(I8Args p) {
 #pragma unroll
         for (int j = 0; j < NTL; ++j) acc[i][j] = (i32x4){0, 0, 0, 0};
     if (FUSED) {
-        // TPR threads a row (a power of two, at least a wave), NT / TPR rows at a time
-        const int tpr = p.M >= NWV ? 64 : p.M > NWV / 2 ? 64 : p.M > NWV / 4 ? 128 : p.M > 1 ? NT / 2 : NT;
-        const int wpr = tpr >> 6, t = tid & (tpr - 1), rpp = NT / tpr;
-        for (int r0 = 0; r0 < p.M; r0 += rpp) {
-            const int m = r0 + tid / tpr;
-            const bool in = m < p.M;
-            const char* row = (const char*)p.x + (size_t)(in ? m : 0) * p.ldx * (FUSED == 2 ? 2 : 4);
-            f8 v[2];                                       // (two groups of eight a thread stay in registers; more come from the cache again)
-            float top = 0.f;
+        // up to NWV rows, each by as many waves as there are for it (a power of two)
+        const int tpr = NT >> (p.M > 4 ? 3 : p.M > 2 ? 2 : p.M > 1 ? 1 : 0), wpr = tpr >> 6, t = tid & (tpr - 1), m = tid / tpr;
+        const bool in = m < p.M;
+        const char* row = (const char*)p.x + (size_t)(in ? m : 0) * p.ldx * (FUSED == 2 ? 2 : 4);
+        f8 v[2];                                           // (two groups of eight a thread stay in registers; more come from the cache again)
+        float top = 0.f;
 #pragma unroll
-            for (int c = 0; c < 2; ++c) { const int i = (c * tpr + t) * 8; if (i < p.S * 64) { v[c] = act8<FUSED == 2>(row, i, p.K, p.xvec); top = top8(v[c], top); } }
-            for (int i = (2 * tpr + t) * 8; i < p.S * 64; i += tpr * 8) top = top8(act8<FUSED == 2>(row, i, p.K, p.xvec), top);
-            top = wave_max(top);
-            if (wpr > 1) {                                 // (uniform over the workgroup)
-                __syncthreads();
-                if (lane == 0) red[wave] = top;
-                __syncthreads();
-                const int w0 = wave & ~(wpr - 1);
-                for (int w = 0; w < wpr; ++w) top = fmaxf(top, red[w0 + w]);
-            }
-            if (in) {
-                if (t == 0) sxs[m] = top / 127.0f;
-                const float inv = 127.0f / top;
-                char* q = xq + m * ldq;
+        for (int c = 0; c < 2; ++c) { const int i = (c * tpr + t) * 8; if (i < p.S * 64) { v[c] = act8<FUSED == 2>(row, i, p.K, p.xvec); top = top8(v[c], top); } }
+        for (int i = (2 * tpr + t) * 8; i < p.S * 64; i += tpr * 8) top = top8(act8<FUSED == 2>(row, i, p.K, p.xvec), top);
+        top = wave_max(top);
+        if (wpr > 1) {                                     // (uniform over the workgroup)
+            if (lane == 0) red[wave] = top;
+            __syncthreads();
+            const int w0 = wave & ~(wpr - 1);
+            for (int w = 0; w < wpr; ++w) top = fmaxf(top, red[w0 + w]);
+        }
+        if (in) {
+            if (t == 0) sxs[m] = top / 127.0f;
+            const float inv = 127.0f / top;
+            char* q = xq + m * ldq;
 #pragma unroll
-                for (int c = 0; c < 2; ++c) { const int i = (c * tpr + t) * 8; if (i < p.S * 64) *(uint2*)(q + i) = quant8(v[c], top, inv); }
-                for (int i = (2 * tpr + t) * 8; i < p.S * 64; i += tpr * 8) *(uint2*)(q + i) = quant8(act8<FUSED == 2>(row, i, p.K, p.xvec), top, inv);
-            }
+            for (int c = 0; c < 2; ++c) { const int i = (c * tpr + t) * 8; if (i < p.S * 64) *(uint2*)(q + i) = quant8(v[c], top, inv); }
+            for (int i = (2 * tpr + t) * 8; i < p.S * 64; i += tpr * 8) *(uint2*)(q + i) = quant8(act8<FUSED == 2>(row, i, p.K, p.xvec), top, inv);
         }
     }
     __syncthreads();
@@ -427,8 +432,8 @@ template <int MT, int NTL, int NWV, int D> static int i8_rows_launch(const I8Arg
     E2T_LAUNCH_CHECK(); return E2T_OK;
 }
 // Which instance: the one whose predicted time is the shortest.  The predictions (microseconds; S = 64-byte k-blocks, W = tiles) are straight
-// lines through measured times of every instance at 90 shapes, M 1 .. 8704, N 200 .. 16384, K 100 .. 16384; over those shapes the choice
-// lies within 8 % of the best instance for three in four and within 25 % for all but a few.  Both sides of the larger steps:
+// lines through measured times of every instance at 120 shapes, M 16 .. 8704, N 100 .. 16384, K 64 .. 16384; over 110 other shapes, M from 1,
+// the chosen instance takes 3 % more than the best one on average and 30 % at most.  Both sides of the larger steps:
 //   M = 16, 4096 x 4096: rows 5.7, 64 x 64 tiles 14.3;   M = 128: rows 12.9, tiles in two K groups 13.0;   M = 256: rows 18.9, tiles 13.5
 //   M = 1024, 4096 x 4096: 64 x 64 39, 128 x 128 31, 128 x 128 in two K groups 26, 256 x 256 51;   M = 4096: 128 x 128 89, 256 x 256 63
 static int i8_launch(const I8Args& p, void* stream) {
@@ -436,10 +441,10 @@ static int i8_launch(const I8Args& p, void* stream) {
     auto cdiv = [](long long a, long long b) { return (double)((a + b - 1) / b); };
     struct { double us; int kind; } best = {1e30, 0};
     auto take = [&](double us, int kind) { if (us < best.us) { best.us = us; best.kind = kind; } };
-    // few rows: start and reduction, then the longest of a wave's chain of steps, the workgroups' reads (9 TB/s) and the weights' from memory
+    // few rows: start and reduction, then the longest of a wave's chain of steps, the workgroups' reads (12 TB/s) and the weights' from memory
     auto rows = [&](int mt, int ntl, int nwv, double step, int kind) {
         const double mb = cdiv(p.M, mt * 16), blocks = cdiv(p.N, ntl * 16) * mb, am = p.M < mt * 16 ? p.M : mt * 16;
-        const double l2 = blocks * (am + ntl * 16) * K64 / 9e6, mem = bytes / 5e6 * (bytes > 3e7 ? mb : 1);
+        const double l2 = blocks * (am + ntl * 16) * K64 / 1.2e7, mem = bytes / 5e6 * (bytes > 3e7 ? mb : 1);
         take(2.2 + 0.5 * mt * ntl + (nwv == 8 ? 0.2 : 0) + fmax(fmax(l2, mem), S / nwv * step), kind);
     };
     if (p.M <= 512) {
@@ -447,15 +452,15 @@ static int i8_launch(const I8Args& p, void* stream) {
     }
     // tiles: the latency of one tile, or the chip's throughput where they queue up
     auto tiles = [&](int t, double step, double fill, double per_step, double per_tile, double base, int kind) {
-        const double W = cdiv(p.M, t) * cdiv(p.N, t);
-        take(fmax(fmax(step * S + fill, per_step * W * S + per_tile * W + base), 2.7 + bytes / 5e6), kind);
+        const double W = cdiv(p.M, t) * cdiv(p.N, t), even = W + 0.66 * (256.0 * ceil(W / 256) - W);      // (some CUs have a tile more than others)
+        take(fmax(fmax(step * S + fill, per_step * even * S + per_tile * W + base), 2.7 + bytes / 5e6), kind);
         return W;
     };
-    if (tiles(64, 0.20, 4.2, 0.00047, 0.003, 4.0, 6) <= 256) take(fmax(0.13 * S + 5.0, 2.7 + bytes / 5e6), 7);
-    if (tiles(128, 0.36, 7.5, 0.0013, 0.004, 5.0, 8) <= 256) take(fmax(0.27 * S + 8.5, 2.7 + bytes / 5e6), 9);
+    if (tiles(64, 0.20, 4.2, 0.0006, 0.0012, 4.0, 6) <= 256) take(fmax(0.13 * S + 5.0, 2.7 + bytes / 5e6), 7);
+    if (tiles(128, 0.36, 7.5, 0.0011, 0.0064, 5.0, 8) <= 256) take(fmax(0.27 * S + 8.5, 2.7 + bytes / 5e6), 9);
     {
         const double W = cdiv(p.M, 256) * cdiv(p.N, 256), left = W < 256 ? 0 : W - 256 * floor(W / 256);
-        const double round = W < 256 ? 0.7 * S + 11 : 0.9 * S + 8;
+        const double round = W < 256 ? 0.7 * S + 11 : 0.85 * S + 13;
         take((W < 256 ? 1 : floor(W / 256)) * round + (left == 0 ? 0 : left <= I8_QUARTERED ? 0.27 * round : round), 10);
     }
     switch (best.kind) {
@@ -511,7 +516,7 @@ static I8Args i8_args(const int8_t* B, long long ldb, const float* sb, const flo
     p.B = B; p.sb = sb; p.bias = bias; p.C = C; p.ldb = ldb; p.ldc = ldc;
     p.M = M; p.N = N; p.K = K; p.S = (K + 63) / 64; p.relu = (flags & E2T_GEMM_RELU) != 0; p.out_bf16 = (flags & E2T_GEMM_OUT_BF16) != 0;
     const unsigned long long al = (unsigned long long)(ldc * (p.out_bf16 ? 2 : 4)) | (uintptr_t)C;
-    p.vec = (al & 15) == 0 ? 16 : (al & 7) == 0 ? 8 : (al & 3) == 0 ? 4 : 2;
+    p.vec = (al & 15) == 0 ? 16 : (al & 7) == 0 ? 8 : (al & 3) == 0 ? 4 : 0;
     return p;
 }
 extern "C" int e2t_gemm_nt_i8(const int8_t* A, long long lda, const float* sa, const int8_t* B, long long ldb, const float* sb,
@@ -524,18 +529,22 @@ extern "C" int e2t_gemm_nt_i8(const int8_t* A, long long lda, const float* sa, c
 }
 
 static inline size_t lin_q_bytes(int M, int K) { return ((size_t)M * (size_t)((K + 63) & ~63) + 255) & ~(size_t)255; }
-// one launch where quantising again in every workgroup costs less than a launch of its own (M = 1: 4096 x 4096 7.1 against 9.3 us,
-// M = 2 8.5 / 9.3, M = 4 10.8 / 9.4; 1806 x 800: M = 8 6.1 / 6.6, M = 16 8.7 / 6.6)
-static bool lin_fused(int M, int K) {
-    return (M == 1 || (M <= 16 && (long long)M * K <= 8192)) && (size_t)M * (((K + 63) & ~63) + 16) <= 100 * 1024;
+// One launch where quantising again in every workgroup (16 outputs each) costs less than a launch of its own: N = 1806 .. 4096, us for one / two
+// launches: M = 1, K = 4096 5.5 / 8.0; M = 2, K = 8192 10.8 / 12; M = 4, K = 2048 6.2 / 6.5, K = 4096 9.4 / 8.5; M = 8, K = 1024 5.8 / 6.0; M = 13,
+// K = 624 8.5 / 6.2.  Many outputs: N = 9000, M = 1, K = 2048 6.5 / 7.5; N = 16384 9.6 / 9.0, K = 4096 14.6 / 16.0; M = 2 18 / 16.
+static bool lin_fused(int M, int N, int K) {
+    if ((size_t)M * (((K + 63) & ~63) + 16) > 100 * 1024) return false;
+    return N > 8192 ? M == 1 && (K >= 4096 || N <= 12288) : M <= 2 || (M <= 8 && M * K <= 8192);
 }
-extern "C" size_t e2t_linear_i8_ws_bytes(int M, int K) { return M > 0 && K > 0 && !lin_fused(M, K) ? lin_q_bytes(M, K) + (size_t)M * sizeof(float) : 0; }
+extern "C" size_t e2t_linear_i8_ws_bytes(int M, int N, int K) {
+    return M > 0 && N > 0 && K > 0 && !lin_fused(M, N, K) ? lin_q_bytes(M, K) + (size_t)M * sizeof(float) : 0;
+}
 extern "C" int e2t_linear_i8(const void* x, int dtype, long long ldx, const int8_t* W, long long ldw, const float* sw, const float* bias, void* y,
                              long long ldy, int M, int N, int K, int flags, void* ws, size_t ws_bytes, void* stream) {
     if (int rc = gemm_i8_check(W, ldw, sw, y, ldy, M, N, K, flags)) return rc;
-    E2T_CHECK_ARG((ws || lin_fused(M, K)) && ws_bytes >= e2t_linear_i8_ws_bytes(M, K) && ((uintptr_t)ws & 15) == 0);
+    E2T_CHECK_ARG((ws || lin_fused(M, N, K)) && ws_bytes >= e2t_linear_i8_ws_bytes(M, N, K) && ((uintptr_t)ws & 15) == 0);
     E2T_CHECK_ARG(x && ldx >= K && (dtype == E2T_DT_F32 || dtype == E2T_DT_BF16) && ((uintptr_t)x & (dtype == E2T_DT_F32 ? 3 : 1)) == 0);
-    if (lin_fused(M, K)) {
+    if (lin_fused(M, N, K)) {
         I8Args p = i8_args(W, ldw, sw, bias, y, ldy, M, N, K, flags);
         p.x = x; p.ldx = ldx; p.xbf16 = dtype == E2T_DT_BF16; p.xvec = (((uintptr_t)x | (unsigned long long)(ldx * (p.xbf16 ? 2 : 4))) & 15) == 0;
         return i8_fused_launch<1, 8, 4>(p, stream);

@@ -282,7 +282,7 @@ class DecodingMixin:
             kin = pr.in_ld if i == 0 else rk(pr.sizes[i])
             if last and q8 is not None:
                 fin = pr.sizes[i]
-                need = lib.e2t_linear_i8_ws_bytes(B, fin)
+                need = lib.e2t_linear_i8_ws_bytes(B, fout, fin)
                 if need and 'i8' not in pw:
                     pw['i8'] = torch.empty(need, dtype=torch.uint8, device=self.device)
                 lib.e2t_linear_i8(cur, DT_BF16, ld, q8[0].data_ptr(), q8[0].shape[1], q8[1].data_ptr(), pr.bias_ptr(i, src),

@@ -154,7 +154,7 @@ def linear_i8(x, w, bias=None, out_dtype=torch.float32, relu=False, out=None):
     n, b, flags = _weights(w, cols, bias, out_dtype, relu, index)
     y, ldy = _out(out, m, n, out_dtype, x)
     if m:
-        need = _c.e2t_linear_i8_ws_bytes(m, cols)
+        need = _c.e2t_linear_i8_ws_bytes(m, n, cols)
         ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
         _call(index, _c.e2t_linear_i8, x.data_ptr(), _DTYPE[x.dtype], ldx, w.q.data_ptr(), w.ld, w.scale.data_ptr(), b, y.data_ptr(), ldy,
               m, n, cols, flags, ws.data_ptr() if need else None, need)

@@ -40,8 +40,8 @@ def test_gemm_refusals(H):
 
 
 def test_linear_refusals(H):
-    f, n = H.lib.e2t_linear_i8, H.lib.e2t_linear_i8_ws_bytes(200, 100)
-    assert n >= 200 * 128 + 800 and H.lib.e2t_linear_i8_ws_bytes(0, 5) == 0
+    f, n = H.lib.e2t_linear_i8, H.lib.e2t_linear_i8_ws_bytes(200, 50, 100)
+    assert n >= 200 * 128 + 800 and H.lib.e2t_linear_i8_ws_bytes(0, 7, 5) == 0
     good = [0x10000, 1, 100, 0x30000, 128, 0x40000, None, 0x50000, 50, 200, 50, 100, 0, 0x60000, n, None]
     for i, v in ((0, None), (0, 0x10001), (1, 5), (2, 99), (3, None), (3, 0x30008), (4, 120), (5, None), (7, None), (8, 49), (9, 0), (10, 0), (11, 0), (11, 131072),
                  (12, 32), (13, None), (13, 0x60004), (14, n - 1)):
