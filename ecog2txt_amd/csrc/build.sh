@@ -28,6 +28,14 @@ for p in "${pids[@]:-}"; do [ -n "$p" ] && wait "$p"; done
 objs=()
 for s in "${srcs[@]}"; do objs+=("$obj/$s.o"); done
 hipcc --offload-arch=gfx950 -fPIC -shared "${objs[@]}" -ldl -o "$out"
+# host side of the tensor-level serving calls: a CPython extension on torch's C++ tensors (no GPU code)
+so="$here/../_serving_host.so"
+if [ ! -f "$so" ] || [ "$here/serving_host.cpp" -nt "$so" ] || [ "$here/build.sh" -nt "$so" ] || [ "$inc/ecog2txt_hip.h" -nt "$so" ]; then
+    py="$(python3 -c 'import sysconfig; print(sysconfig.get_paths()["include"])')"
+    torch="$(python3 -c 'import importlib.util as u; print(u.find_spec("torch").submodule_search_locations[0])')"
+    g++ -O2 -std=c++17 -fPIC -shared -Wall -I"$inc" -I"$py" -isystem "$torch/include" -isystem "$torch/include/torch/csrc/api/include" "$here/serving_host.cpp" -o "$so" \
+        -L"$torch/lib" -lc10 -ltorch_cpu -ltorch_python > "$obj/serving_host.log" 2>&1 || { head -40 "$obj/serving_host.log"; exit 1; }
+fi
 echo "built $out"
 # test helper (tests/native/occupy.hip: a CU-occupying spin kernel for the RCCL-contention test) -- not part of the product library
 th="$here/../../tests/native"

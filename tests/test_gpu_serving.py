@@ -401,6 +401,45 @@ def test_sample_rows_does_not_depend_on_the_batch(S):
 
 
 # ---------------------------------------------------------------------------------------------------- one step of a decoder's head
+def test_refused_tensors(S):
+    """What the tensor-level calls refuse, with the references they took given back."""
+    import sys
+    dev = 'cuda'
+    x, w = torch.randn(3, 100, device=dev), S.quantize_rows(torch.randn(50, 100, device=dev))
+    a, bias, u = S.quantize_rows(x), torch.zeros(50, device=dev), torch.zeros(3, device=dev)
+    q = torch.zeros(4, 128, dtype=torch.int8, device=dev)
+    ones = torch.ones(4, device=dev)
+    out = torch.empty(3, 50, device=dev)
+    grad = torch.randn(3, 100, device=dev, requires_grad=True)
+    calls = [lambda: S.quantize_rows(x.half()), lambda: S.quantize_rows(x[0]), lambda: S.quantize_rows(x.t()), lambda: S.quantize_rows(x[:, :0]),
+             lambda: S.quantize_rows(x[:1].expand(3, 100)), lambda: S.quantize_rows(grad), lambda: S.quantize_rows(None),
+             lambda: S.Int8Rows(q, ones, 129), lambda: S.Int8Rows(q, ones, 0), lambda: S.Int8Rows(q, ones[:3], 100), lambda: S.Int8Rows(q, ones.double(), 100),
+             lambda: S.Int8Rows(q[:, 1:], ones, 64), lambda: S.Int8Rows(q[:, :100], ones, 100), lambda: S.Int8Rows(q.int(), ones, 100),
+             lambda: S.matmul_i8(x, w), lambda: S.matmul_i8(a, x), lambda: S.matmul_i8(a, S.quantize_rows(x[:, :64])), lambda: S.matmul_i8(a, w, bias[:49]),
+             lambda: S.matmul_i8(a, w, bias.bfloat16()), lambda: S.matmul_i8(a, w, bias.cpu()), lambda: S.matmul_i8(a, w, out_dtype=torch.float16),
+             lambda: S.matmul_i8(a, w, out_dtype=None), lambda: S.matmul_i8(a, w, out=out[:2]), lambda: S.matmul_i8(a, w, out=out, out_dtype=torch.bfloat16),
+             lambda: S.matmul_i8(a, w, out=out.t()), lambda: S.linear_i8(x[:, :99], w), lambda: S.linear_i8(grad, w), lambda: S.linear_i8(x, w, bias[None]),
+             lambda: S.linear_i8(x, w, out=x), lambda: S.sample_rows(x.int(), u), lambda: S.sample_rows(x, u[:2]), lambda: S.sample_rows(x, u.double()),
+             lambda: S.sample_rows(x, u.cpu()), lambda: S.sample_rows(x, u, temperature=u.double()), lambda: S.sample_rows(x, u, top_k=u),
+             lambda: S.sample_rows(x, u, top_p=u[:2]), lambda: S.sample_rows(x, u, min_p=u[:, None])]
+    held = [x, w.q, w.scale, a.q, a.scale, bias, u, q, ones, out]
+    before = [sys.getrefcount(t) for t in held]
+    for c in calls:
+        for _ in range(3):
+            with pytest.raises(ValueError):
+                c()
+    for bad in (dict(top_k='a'), dict(temperature=None), dict(min_p=[1])):
+        with pytest.raises((TypeError, ValueError)):
+            S.sample_rows(x, u, **bad)
+    for _ in range(3):
+        S.linear_i8(x, w, bias), S.matmul_i8(a, w, bias, out=out), S.sample_rows(x, u, top_k=10 ** 30, top_p=0.5), S.sample_rows(x, u, top_k=-10 ** 30)
+    assert [sys.getrefcount(t) for t in held] == before
+    with torch.no_grad():
+        S.linear_i8(grad, w)
+    assert S.matmul_i8(S.quantize_rows(x[:0]), w).shape == (0, 50) and S.linear_i8(x[:0], w, bias).shape == (0, 50)
+    assert [t.shape for t in S.sample_rows(x[:0], u[:0])] == [(0,), (0,)]
+
+
 def test_head_of_a_decoder_step_in_a_graph_and_on_two_streams(S):
     """quantise + product + draw as a decoding service runs them: eager, captured and replayed with new inputs, two streams at once."""
     M, V, K = 48, 1806, 800
