@@ -269,20 +269,22 @@ __device__ __forceinline__ void sample_store(const SampleArgs& a, int b, int tok
 __device__ __forceinline__ float log_prob(const Weigh& w, double at, u64 all) { return (float)(at * (-1.0 / 64.0) - log((double)all / w.scale)); }
 
 // ---- ranking a few tokens among themselves -----------------------------------------------------------------------------------------
-// Of the tokens with rank <= hi that `each` enumerates (at most n, each by exactly one thread): the need-th by count (BY_MASS false; there are
+// Of the tokens with rank <= hi that `each` enumerates (at most n, each by exactly one thread): the need-th by count (by_mass false; there are
 // as many), or the first at which the running mass reaches need -- the last one where the whole does not; `mass_to`: the mass up to
 // and with it.  While there are more than 64: a histogram over the eight highest bits in which they differ.  The rest lie in a list, a lane
 // each, and every wave ranks them for itself against the lanes' values: no barrier behind the one that completes the list (as one
 // list for the workgroup with n^2 comparisons spread over it: 2.2 us a call, most of it barriers and LDS round trips).
-// One call each of either kind in a kernel; L.n is zero at the first.
+// One call each of either kind in a kernel, from one place (inlined twice, the code of a kernel grows by a third, and between other kernels it is
+// fetched anew each time); L.n is zero at the first.
+struct Found { u64 before, mass; int bin, count; };            // the bin that holds a cut: tokens and mass in front of it, tokens in it
 template <int NT> struct SelectLds {
     u64 m[256]; unsigned c[256];
     u64 list[2][64];
     unsigned n[2];
     u64 out[3];
 };
-template <int NT, bool BY_MASS, class Each> __device__ __forceinline__ u64 select_rank(Each each, u64 hi, int n, u64 need, const Weigh& w, SelectLds<NT>& L, u64* red,
-                                                                                      u64& mass_to) {
+template <int NT, class Each> __device__ __forceinline__ u64 select_rank(Each each, u64 hi, int n, u64 need, bool by_mass, const Weigh& w, SelectLds<NT>& L, u64* red,
+                                                                        u64& mass_to) {
     u64 lo = 0, before_m = 0, before_c = 0;
     while (__builtin_expect(n > 64, 0)) {
         u64 mn = ~0ull, mx = ~0ull;
@@ -302,7 +304,7 @@ template <int NT, bool BY_MASS, class Each> __device__ __forceinline__ u64 selec
         u64 tc, tm, bc = mc, bm = mm;
         block_scan2<NT>(bc, bm, red, tc, tm);
         bc += before_c; bm += before_m;
-        const u64 b = BY_MASS ? bm : bc, x = BY_MASS ? mm : mc, most = BY_MASS ? before_m + tm : before_c + tc, nd = need < most ? need : most;
+        const u64 b = by_mass ? bm : bc, x = by_mass ? mm : mc, most = by_mass ? before_m + tm : before_c + tc, nd = need < most ? need : most;
         if (threadIdx.x < 256 && b < nd && b + x >= nd) { L.out[0] = threadIdx.x; L.out[1] = bc; L.out[2] = bm; }
         __syncthreads();
         const u64 d = L.out[0];
@@ -312,10 +314,10 @@ template <int NT, bool BY_MASS, class Each> __device__ __forceinline__ u64 selec
         n = (int)L.c[d];
         __syncthreads();
     }
-    u64* list = L.list[BY_MASS];
-    each([&](u64 r) { if (r >= lo && r <= hi) { const unsigned k = atomicAdd(&L.n[BY_MASS], 1u); if (k < 64) list[k] = r; } });
+    u64* list = L.list[by_mass];
+    each([&](u64 r) { if (r >= lo && r <= hi) { const unsigned k = atomicAdd(&L.n[by_mass], 1u); if (k < 64) list[k] = r; } });
     __syncthreads();
-    n = __builtin_amdgcn_readfirstlane((int)L.n[BY_MASS]);
+    n = __builtin_amdgcn_readfirstlane((int)L.n[by_mass]);
     if (n == 0) { mass_to = before_m; return ~0ull; }
     const int lane = threadIdx.x & 63;
     const u64 r = lane < n ? list[lane] : ~0ull, own = lane < n ? w.mass(w.at(rank_value(r))) : 0;
@@ -329,8 +331,8 @@ template <int NT, bool BY_MASS, class Each> __device__ __forceinline__ u64 selec
         }
     }
     const int last = __ffsll((unsigned long long)__ballot(lane < n && c == (unsigned)n)) - 1;
-    const u64 most = lane_u64(m, last), nd = BY_MASS && need > most ? most : need;
-    const u64 x = BY_MASS ? m : before_c + c, b = BY_MASS ? x - own : x - 1;
+    const u64 most = lane_u64(m, last), nd = by_mass && need > most ? most : need;
+    const u64 x = by_mass ? m : before_c + c, b = by_mass ? x - own : x - 1;
     const u64 hit = __ballot(lane < n && b < nd && x >= nd);
     const int at = hit ? __ffsll(hit) - 1 : last;
     mass_to = lane_u64(m, at);
@@ -338,8 +340,8 @@ template <int NT, bool BY_MASS, class Each> __device__ __forceinline__ u64 selec
 }
 
 // ---- one workgroup a row ---------------------------------------------------------------------------------------------------------------
-// (The histogram here is of 512 bins of 1/16, counts and masses apart: two bins a thread or one, no conversions, and the masses stay
-// in registers for the draw: 1806 tokens with all four settings in 7.4 us, 256 such rows in 8.6.  It is a chain of dependent steps: load 0.7,
+// (The histogram here is of 512 bins over the row's spread, counts and masses apart: two bins a thread or one, no conversions, and the
+// masses stay in registers for the draw: 1806 tokens with all four settings in 7.2 us, 256 such rows in 8.4.  It is a chain of dependent steps: load 0.7,
 // maximum 0.3, masses and bins 1.3, each cut 1.5, draw and logarithm 1.4.)
 template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sample_row(SampleArgs a) {
     constexpr int E = Row<BF16>::E, NG = VPT / E, NB = 512, PER = NB / NT, NW = NT / 64;
@@ -348,7 +350,7 @@ template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sa
     __shared__ u64 hist_m[NB];
     __shared__ unsigned hist_c[NB];
     __shared__ SelectLds<NT> L;
-    __shared__ u64 zs[6];
+    __shared__ Found found[2];
     const int b = blockIdx.x, tid = threadIdx.x;
     const Row<BF16> row(a, b);
     // thread t holds tokens t * VPT - o .. + VPT - 1
@@ -364,10 +366,16 @@ template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sa
     float v[VPT];
 #pragma unroll
     for (int q = 0; q < NG; ++q) row.unpack(raw[q], v + q * E);
-    float top = v[0];
+    float top = -INFINITY, low = -INFINITY;                // the largest, and minus the smallest that can be drawn
 #pragma unroll
-    for (int j = 1; j < VPT; ++j) top = fmaxf(top, v[j]);
-    top = block_max<NT, true>(top, red);                   // (its barrier publishes the table and the empty histogram)
+    for (int j = 0; j < VPT; ++j) { top = fmaxf(top, v[j]); low = fmaxf(low, v[j] == -INFINITY ? -INFINITY : -v[j]); }
+    top = wave_max_63(top); low = wave_max_63(low);
+    float* tops = (float*)red;
+    if ((tid & 63) == 63) { tops[2 * (tid >> 6)] = top; tops[2 * (tid >> 6) + 1] = low; }
+    __syncthreads();                                       // (publishes the table and the empty histogram, too)
+    top = tops[0]; low = tops[1];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) { top = fmaxf(top, tops[2 * i]); low = fmaxf(low, tops[2 * i + 1]); }
     if (top == -INFINITY) { if (tid == 0) sample_store(a, b, -1, -INFINITY); return; }
     if (st.greedy) {
         u64 best = ~0ull;
@@ -385,10 +393,11 @@ template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sa
     int ci = 0x7FFFFFFF;
     if (st.use_k || st.use_p) {
         short bin[VPT];
+        const double spread = fmin(w.at(-low), (double)SMP_BINS), fine = spread > 0.0 ? 0.999999 * NB / spread : 0.0;      // (a flat row's tokens in few bins: 15 us instead of 7.9)
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             const double at = w.at(v[j]);
-            const int n = at < (double)SMP_BINS ? (int)(at * ((double)NB / SMP_BINS)) : NB;
+            const int n = at < (double)SMP_BINS ? (int)(at * fine) : NB;
             bin[j] = (short)n;
             if (n < NB) { atomicAdd(&hist_c[n], 1u); atomicAdd(&hist_m[n], tm[j]); }
         }
@@ -396,40 +405,34 @@ template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sa
         u64 c[PER], m[PER], cs = 0, ms = 0;
 #pragma unroll
         for (int j = 0; j < PER; ++j) { c[j] = hist_c[tid * PER + j]; m[j] = hist_m[tid * PER + j]; cs += c[j]; ms += m[j]; }
-        u64 call, mass, cb = cs, mb = ms;
+        u64 call, mass, cb = cs, mb = ms, cut = ~0ull;
         block_scan2<NT, true>(cb, mb, red + NW, call, mass);
-        // tokens of one bin, by rank
-        auto in_bin = [&](int n) {
-            return [&, n](auto f) {
-#pragma unroll
-                for (int j = 0; j < VPT; ++j) if (bin[j] == n) f(rank_of(v[j], i0 + j));
-            };
-        };
-        u64 cut = ~0ull;
-        if (st.use_k && (u64)st.k < call) {
+        const bool cut_k = st.use_k && (u64)st.k < call;
+#pragma clang loop unroll(disable)
+        for (int by_mass = 0; by_mass < 2; ++by_mass) {    // top-k, then top-p of what it leaves
+            if (by_mass ? !st.use_p : !cut_k) continue;
+            const u64 need = by_mass ? p_need(st.P, mass) : (u64)st.k;       // (at most the mass, or the count: a bin holds it)
             u64 cc = cb, mm = mb;
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
-                if (cc < (u64)st.k && cc + c[j] >= (u64)st.k) { zs[0] = (u64)(tid * PER + j); zs[2] = cc | (c[j] << 32); zs[3] = mm; }
+                const u64 b = by_mass ? mm : cc, x = by_mass ? m[j] : c[j];
+                if (b < need && b + x >= need) found[by_mass] = {cc, mm, tid * PER + j, (int)c[j]};
                 cc += c[j]; mm += m[j];
             }
             __syncthreads();
-            const u64 before = zs[2] & 0xFFFFFFFFull, above = zs[3];
-            u64 to;
-            cut = select_rank<NT, false>(in_bin((int)zs[0]), ~0ull, (int)(zs[2] >> 32), (u64)st.k - before, w, L, red + 3 * NW, to);
-            mass = above + to;
-        }
-        if (st.use_p) {
-            const u64 need = p_need(st.P, mass);           // (at most the mass: a bin holds it)
-            u64 mm = mb;
+            const Found f = found[by_mass];
+            auto in_bin = [&](auto g) {                    // its tokens, by rank
 #pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                if (mm < need && mm + m[j] >= need) { zs[1] = (u64)(tid * PER + j); zs[4] = c[j]; zs[5] = mm; }
-                mm += m[j];
-            }
-            __syncthreads();
+                for (int j = 0; j < VPT; ++j) {
+                    if (bin[j] != f.bin) continue;
+                    float x = v[j];
+                    asm volatile("" : "+v"(x));            // (the few that are there; not all ranks ahead of the loop)
+                    g(rank_of(x, i0 + j));
+                }
+            };
             u64 to;
-            cut = select_rank<NT, true>(in_bin((int)zs[1]), cut, (int)zs[4], need - zs[5], w, L, red + 3 * NW, to);
+            cut = select_rank<NT>(in_bin, cut, f.count, need - (by_mass ? f.mass : f.before), by_mass, w, L, red + 3 * NW, to);
+            mass = f.mass + to;
         }
         if (cut != ~0ull) { cv = rank_value(cut); ci = (int)(unsigned)cut; }
     }
@@ -437,6 +440,7 @@ template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sa
     u64 s = 0;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
+        asm volatile("" : "+v"(v[j]));                     // (nothing kept from above but logits and masses)
         const bool in = v[j] > cv || (v[j] == cv && i0 + j <= ci);
         tm[j] = in && (!st.use_m || w.at(v[j]) <= w.amax) ? tm[j] : 0;
         s += tm[j];
@@ -770,7 +774,8 @@ template <bool BF16> __global__ __launch_bounds__(512) void k_sample_draw(Sample
     __shared__ u64 tsum[SMP_TILES_MAX];
     __shared__ u64 sub_m[SMP_SUB];
     __shared__ unsigned sub_c[SMP_SUB];
-    __shared__ u64 zs[4];
+    __shared__ Found found[2];
+    __shared__ u64 zs[2];
     const int b = blockIdx.x, tid = threadIdx.x;
     const RowWs ws = row_ws(a, b);
     const ZoneRec rec = *ws.rec;
@@ -790,7 +795,7 @@ template <bool BF16> __global__ __launch_bounds__(512) void k_sample_draw(Sample
     const Weigh w(&tab, rec.top, rec.s, rec.amax, a.frac);
     if (tid < a.tiles) tsum[tid] = tile_kept;
     if (cuts) for (int i = tid; i < SMP_SUB; i += NT) { sub_m[i] = 0; sub_c[i] = 0; }
-    if (tid == 0) zs[0] = zs[1] = ~0ull;
+    if (tid == 0) found[1].bin = -1;
     __syncthreads();
     u64 cut = ~0ull;
     if (cuts) {
@@ -839,36 +844,26 @@ template <bool BF16> __global__ __launch_bounds__(512) void k_sample_draw(Sample
         u64 cb = cs, mb = ms, xc;
         block_scan2<NT, true>(cb, mb, red, xc, x);
         cb += above_c; mb += above;
-        u64 to, mass = rec.whole;
-        if (rec.cut_k) {
+        u64 mass = rec.whole;
+        const u64 most = above + x;
+#pragma clang loop unroll(disable)
+        for (int by_mass = 0; by_mass < 2; ++by_mass) {    // top-k, then top-p of what it leaves
+            if (by_mass ? !rec.cut_p : !rec.cut_k) continue;
+            const u64 nd = by_mass ? p_need(rec.P, mass) : 0;
+            const u64 need = !by_mass ? (u64)rec.k : nd > most ? most : nd > above ? nd : above + 1;
             u64 cc = cb, mm = mb;
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
-                if (cc < (u64)rec.k && cc + c[j] >= (u64)rec.k) { zs[0] = (u64)(tid * PER + j); zs[2] = cc; zs[3] = mm; }
+                const u64 b = by_mass ? mm : cc, y = by_mass ? m[j] : c[j];
+                if (b < need && b + y >= need) found[by_mass] = {cc, mm, tid * PER + j, (int)c[j]};
                 cc += c[j]; mm += m[j];
             }
             __syncthreads();
-            const int i = (int)zs[0];
-            const u64 cf = zs[2], mf = zs[3];
-            cut = select_rank<NT, false>(in_sub(i), ~0ull, (int)sub_c[i], (u64)rec.k - cf, w, L, red + 2 * (NT / 64), to);
-            mass = mf + to;
-        }
-        if (rec.cut_p) {
-            const u64 most = above + x;
-            const u64 nd = p_need(rec.P, mass), need = nd > most ? most : nd > above ? nd : above + 1;
-            u64 mm = mb;
-            __syncthreads();
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                if (mm < need && mm + m[j] >= need) { zs[1] = (u64)(tid * PER + j); zs[2] = mm; }
-                mm += m[j];
-            }
-            __syncthreads();
-            if (zs[1] != ~0ull) {                          // (else the zone's tokens weigh nothing: no matter which are kept)
-                const int i = (int)zs[1];
-                const u64 cp = select_rank<NT, true>(in_sub(i), cut, (int)sub_c[i], need - zs[2], w, L, red + 2 * (NT / 64), to);
-                cut = cp < cut ? cp : cut;
-            }
+            const Found f = found[by_mass];
+            if (f.bin < 0) break;                          // (the zone's tokens weigh nothing: no matter which are kept)
+            u64 to;
+            cut = select_rank<NT>(in_sub(f.bin), cut, f.count, need - (by_mass ? f.mass : f.before), by_mass, w, L, red + 2 * (NT / 64), to);
+            mass = f.mass + to;
         }
         auto keep = [&](u64 r, u64 m) { if (r <= cut && w.at(rank_value(r)) <= w.amax) atomicAdd(&tsum[((int)(unsigned)r + row.o) / SMP_TILE], m); };
         if (rec.n <= KEEP * NT) {
