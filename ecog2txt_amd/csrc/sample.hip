@@ -908,7 +908,7 @@ template <bool BF16> __global__ __launch_bounds__(512) void k_sample_draw(Sample
 #define SMP_ROW_MAX (8192 - 7)          // (a row may start up to seven elements behind a 16-byte boundary)
 static int frac_bits(int V) { int c = 0; while ((1ll << c) < V) ++c; return 62 - c < 50 ? 62 - c : 50; }
 static int long_tiles(int V) { return (V + 7 + SMP_TILE - 1) / SMP_TILE; }
-// chunks of a long row: enough workgroups for the chip (1024 in all) but no more than k_sample_zone merges quickly (16, 16 KB each), at most
+// chunks of a long row: enough workgroups for the chip (1024 in all) but no more than k_sample_zone merges quickly (16, 8 KB each), at most
 // SMP_CHUNK_TILES tiles in one
 static int long_chunks(int B, int V) {
     const int tiles = long_tiles(V), least = (tiles + SMP_CHUNK_TILES - 1) / SMP_CHUNK_TILES;
