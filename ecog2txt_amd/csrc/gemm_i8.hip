@@ -537,7 +537,7 @@ static bool lin_fused(int M, int N, int K) {
     return N > 8192 ? M == 1 && (K >= 4096 || N <= 12288) : M <= 2 || (M <= 8 && M * K <= 8192);
 }
 extern "C" size_t e2t_linear_i8_ws_bytes(int M, int N, int K) {
-    return M > 0 && N > 0 && K > 0 && !lin_fused(M, N, K) ? lin_q_bytes(M, K) + (size_t)M * sizeof(float) : 0;
+    return M > 0 && N > 0 && K > 0 && K <= E2T_I8_MAX_K && !lin_fused(M, N, K) ? lin_q_bytes(M, K) + (size_t)M * sizeof(float) : 0;
 }
 extern "C" int e2t_linear_i8(const void* x, int dtype, long long ldx, const int8_t* W, long long ldw, const float* sw, const float* bias, void* y,
                              long long ldy, int M, int N, int K, int flags, void* ws, size_t ws_bytes, void* stream) {

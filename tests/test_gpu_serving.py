@@ -171,6 +171,25 @@ def test_matmul_i8_strides_and_what_lies_around(S, M, N, K, out):
     assert (frame == -7.0).all()
 
 
+@pytest.mark.parametrize('out', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('M,N,K', [(70, 259, 130), (700, 301, 64), (1100, 1305, 700), (2049, 2310, 200), (4099, 4101, 4104), (1030, 9001, 5000)])
+def test_matmul_i8_rows_that_start_anywhere(S, M, N, K, out):
+    """Every tile size, rows of the output on every alignment: the same values, nothing beside them touched."""
+    a, w = ints(M, K, 1), ints(N, K, 2)
+    acc = a.double() @ w.double().t()                                  # (whole numbers below 2^53: exact)
+    want = acc.float().to(out)
+    A, W = rows_of(S, a), rows_of(S, w)
+    step = 1 if out is torch.bfloat16 else 2
+    for off in range(0, 9, 1 if M < 2000 else 3):
+        for more in (0, 1, 2, 4, 7, 8)[::step]:
+            big = torch.full((M, N + 8 + more), -7.0, dtype=out, device='cuda')
+            y = big[:, off:off + N]
+            assert S.matmul_i8(A, W, out_dtype=out, out=y) is y
+            assert torch.equal(y, want)
+            y.fill_(-7.0)
+            assert (big == -7.0).all()
+
+
 def test_matmul_i8_only_one_operand_needs_zero_padding(S):
     a, b = ints(20, 64, 1), ints(30, 64, 2)
     b[:, 50:] = 0
@@ -347,6 +366,19 @@ def test_sample_rows_levels_on_bin_borders(S, T, unit):
     l = -level * unit
     l[:, 77] = 0
     for kw in (dict(top_k=300), dict(top_k=9000), dict(top_k=V - 5), dict(top_k=30000, top_p=0.83), dict(top_p=0.77), dict(top_k=20000, top_p=0.9, min_p=1e-3)):
+        check_sample(S, l, torch.rand(B, generator=g, device='cuda'), temperature=T, **kw)
+
+
+@pytest.mark.parametrize('V', [3, 40, 1806, 6000, 8185, 8186, 20011])
+@pytest.mark.parametrize('sd,T', [(0.05, 1.0), (1e-4, 1.0), (30.0, 1.0), (1.0, 40.0), (1.0, 1e-3), (1e-30, 1.0), (1e30, 1.0)])
+def test_sample_rows_flat_and_steep(S, V, sd, T):
+    """Spreads from nothing to beyond what weighs anything."""
+    B = 5
+    g = gen(V + int(T))
+    l = torch.randn(B, V, generator=g, device='cuda') * sd
+    l[1, ::2] = float('-inf')
+    l[2] = l[2, 0]
+    for kw in (dict(top_k=2), dict(top_k=50), dict(top_k=V - 1), dict(top_k=V // 2 + 1, top_p=0.7), dict(top_k=7, min_p=0.9)):
         check_sample(S, l, torch.rand(B, generator=g, device='cuda'), temperature=T, **kw)
 
 
