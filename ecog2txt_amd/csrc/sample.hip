@@ -6,11 +6,11 @@
 // Masses are WHOLE NUMBERS: w_i = round(2^F exp(z_i - z_max)), F = min(50, 62 - ceil(log2 V)), the exponential in double precision;
 // what lies 32 or more below the maximum (e^-32 = 1.3e-14) weighs nothing.  Integer sums do not depend on their order: any order of
 // atomics gives the same sums, the same cut and the same token, bit for bit; the draw itself not on the split of the row either (what
-// top_p is a share of does in long rows, by 6e-12: k_sample_hist).  fp32 sums would not do: over a flat vocabulary of 128 k tokens the borders between tokens lie 8e-6 of the whole apart and
-// 6e-8 of rounding moves the answer of one row in a hundred.
+// top_p is a share of does in long rows, by 6e-12: k_sample_hist).  fp32 sums would not do: over a flat vocabulary of 128 k tokens the
+// borders between tokens lie 8e-6 of the whole apart and 6e-8 of rounding moves the answer of one row in a hundred.
 // fp64 multiply-adds run at the rate of unpacked fp32 ones on this chip, and the exponential takes a table entry and a short polynomial.
 //
-// Finding the cut.  A histogram of bins of 1/16 or 1/32 in z (counts and masses) says in which bin the k-th token, or
+// Finding the cut.  A histogram (counts and masses; 512 bins over the row's spread, or bins of 1/32 in z) says in which bin the k-th token, or
 // p of the mass, lies; only that bin's tokens are ranked among themselves.
 //
 // Rows up to SMP_ROW_MAX tokens: one workgroup a row, the row in registers, one launch (k_sample_row).  Longer rows: four launches, the row
@@ -180,7 +180,8 @@ template <int NT, bool OWN = false> __device__ __forceinline__ void block_scan2(
 
 // ---- weights ------------------------------------------------------------------------------------------------------------------------
 // 2^F exp(-at / 64), at >= 0: the nearest whole number's from a table in LDS (made as the product of two short ones; what lies 2048
-// or further down weighs nothing), the rest from a polynomial: about 18 instructions a token, and no branch between the tokens of a thread, so that their chains interleave.
+// or further down weighs nothing), the rest from a polynomial: about 18 instructions a token, and no branch between the tokens of
+// a thread, so that their chains interleave.
 // exp(-n) and exp(-n / 64), rounded to the nearest: loads that travel with the logits', where exp() itself would take 0.5 us
 __device__ const double smp_exp_a[32] = {
     0x1.0000000000000p+0, 0x1.78b56362cef38p-2, 0x1.152aaa3bf81ccp-3, 0x1.97db0ccceb0afp-5, 0x1.2c155b8213cf4p-6, 0x1.b993fe00d5376p-8,
@@ -341,8 +342,8 @@ template <int NT, class Each> __device__ __forceinline__ u64 select_rank(Each ea
 
 // ---- one workgroup a row ---------------------------------------------------------------------------------------------------------------
 // (The histogram here is of 512 bins over the row's spread, counts and masses apart: two bins a thread or one, no conversions, and the
-// masses stay in registers for the draw: 1806 tokens with all four settings in 7.2 us, 256 such rows in 8.4.  It is a chain of dependent steps: load 0.7,
-// maximum 0.3, masses and bins 1.3, each cut 1.5, draw and logarithm 1.4.)
+// masses stay in registers for the draw: 1806 tokens with all four settings in 7.2 us, 256 such rows in 8.4.  It is a chain of dependent
+// steps: load 0.7, maximum 0.3, masses and bins 1.3, each cut 1.5, draw and logarithm 1.4.)
 template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sample_row(SampleArgs a) {
     constexpr int E = Row<BF16>::E, NG = VPT / E, NB = 512, PER = NB / NT, NW = NT / 64;
     __shared__ u64 red[6 * NW];                            // (a place for each reduction)
