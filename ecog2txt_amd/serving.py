@@ -17,8 +17,12 @@ _host = None
 def _bind():
     """The native host module, with the library's functions handed to it (on the first use)."""
     global _host
-    from . import _serving_host as host
     lib = H.load()
+    try:
+        from . import _serving_host as host
+    except ImportError as e:
+        raise RuntimeError('ecog2txt_amd/_serving_host.so is not built or does not fit this torch (%s). Run `python -c "import __graft_entry__ as g; '
+                           'g.build()"` or ecog2txt_amd/csrc/build.sh.' % e) from e
     names = ('e2t_quant_rows_i8', 'e2t_gemm_nt_i8', 'e2t_linear_i8_ws_bytes', 'e2t_linear_i8', 'e2t_sample_ws_bytes', 'e2t_sample_rows', 'e2t_last_error')
     stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
     host.bind({n: C.cast(getattr(lib, n), C.c_void_p).value for n in names}, stream, Int8Rows)
