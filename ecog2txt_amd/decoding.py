@@ -4,9 +4,10 @@ import ctypes as C
 
 import torch
 
-from .hip_lib import DT_BF16, DT_F32, SampleCfg, lib
+from .hip_lib import DT_BF16, DT_F32, lib
 from .params import EOS_ID, PAD_ID, capture, ceil_div, r8, rk
 from .layers import _bf, _f32, _i32
+from .serving import sample_config
 
 
 class DecodingMixin:
@@ -138,8 +139,7 @@ class DecodingMixin:
         B, L = ws['B'], ws['L']
         st = self.stream
         dw, pw, sm = ws['dec'], ws['proj'], ws['sample']
-        cfg = SampleCfg(temperature_rows=sm['temperature'].data_ptr(), top_k_rows=sm['top_k'].data_ptr(), top_p_rows=sm['top_p'].data_ptr(),
-                        min_p_rows=sm['min_p'].data_ptr())
+        cfg = sample_config(B, sm['u'].get_device(), sm['temperature'], sm['top_k'], sm['top_p'], sm['min_p'])
         self.encode(ws, src, False)
         lib.e2t_decode_init(ws['done'].data_ptr(), ws['hyp'].data_ptr(), ws['U'].data_ptr(), ws['dlens'].data_ptr(), B, L, EOS_ID, PAD_ID, st)
         lib.e2t_fill_u32(sm['score'].data_ptr(), B, 0, st)
