@@ -10,7 +10,7 @@
 // borders between tokens lie 8e-6 of the whole apart and 6e-8 of rounding moves the answer of one row in a hundred.
 // fp64 multiply-adds run at the rate of unpacked fp32 ones on this chip, and the exponential takes a table entry and a short polynomial.
 //
-// Finding the cut.  A histogram (counts and masses; 512 bins over the row's spread, or bins of 1/32 in z) says in which bin the k-th token, or
+// Finding the cut.  A histogram (counts and masses; 512 or 1024 bins over the row's spread, or bins of 1/32 in z) says in which bin the k-th token, or
 // p of the mass, lies; only that bin's tokens are ranked among themselves.
 //
 // Rows up to SMP_ROW_MAX tokens: one workgroup a row, the row in registers, one launch (k_sample_row).  Longer rows: four launches, the row
@@ -341,11 +341,12 @@ template <int NT, class Each> __device__ __forceinline__ u64 select_rank(Each ea
 }
 
 // ---- one workgroup a row ---------------------------------------------------------------------------------------------------------------
-// (The histogram here is of 512 bins over the row's spread, counts and masses apart: two bins a thread or one, no conversions, and the
+// (The histogram here is of 512 or 1024 bins over the row's spread, counts and masses apart: two bins a thread or one, no conversions, and the
 // masses stay in registers for the draw: 1806 tokens with all four settings in 7.2 us, 256 such rows in 8.4.  It is a chain of dependent
 // steps: load 0.7, maximum 0.3, masses and bins 1.3, each cut 1.5, draw and logarithm 1.4.)
 template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sample_row(SampleArgs a) {
-    constexpr int E = Row<BF16>::E, NG = VPT / E, NB = 512, PER = NB / NT, NW = NT / 64;
+    constexpr int E = Row<BF16>::E, NG = VPT / E, NB = VPT <= 8 ? 512 : 1024, PER = NB / NT, NW = NT / 64;
+    constexpr bool HOLD = VPT <= 16;                       // masses in registers (32 of them would spill: they are worked out again)
     __shared__ u64 red[6 * NW];                            // (a place for each reduction)
     __shared__ ExpTab tab;
     __shared__ u64 hist_m[NB];
@@ -387,9 +388,12 @@ template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sa
         return;
     }
     const Weigh w(&tab, top, st, a.frac);
-    u64 tm[VPT];
+    u64 tm[HOLD ? VPT : 1];
+    auto mass_of = [&](int j) { return HOLD ? tm[HOLD ? j : 0] : w.mass(w.at(v[j])); };
+    if (HOLD) {
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) tm[j] = w.mass(w.at(v[j]));
+        for (int j = 0; j < VPT; ++j) tm[HOLD ? j : 0] = w.mass(w.at(v[j]));
+    }
     float cv = -INFINITY;                                  // kept: logit above cv, or equal and index up to ci
     int ci = 0x7FFFFFFF;
     if (st.use_k || st.use_p) {
@@ -400,7 +404,7 @@ template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sa
             const double at = w.at(v[j]);
             const int n = at < (double)SMP_BINS ? (int)(at * fine) : NB;
             bin[j] = (short)n;
-            if (n < NB) { atomicAdd(&hist_c[n], 1u); atomicAdd(&hist_m[n], tm[j]); }
+            if (n < NB) { atomicAdd(&hist_c[n], 1u); atomicAdd(&hist_m[n], mass_of(j)); }
         }
         __syncthreads();
         u64 c[PER], m[PER], cs = 0, ms = 0;
@@ -438,13 +442,17 @@ template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sa
         if (cut != ~0ull) { cv = rank_value(cut); ci = (int)(unsigned)cut; }
     }
     // the draw: running sums in the order of the vocabulary
+    auto kept = [&](int j) {
+        const bool in = v[j] > cv || (v[j] == cv && i0 + j <= ci);
+        return in && (!st.use_m || w.at(v[j]) <= w.amax) ? mass_of(j) : 0;
+    };
     u64 s = 0;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
         asm volatile("" : "+v"(v[j]));                     // (nothing kept from above but logits and masses)
-        const bool in = v[j] > cv || (v[j] == cv && i0 + j <= ci);
-        tm[j] = in && (!st.use_m || w.at(v[j]) <= w.amax) ? tm[j] : 0;
-        s += tm[j];
+        const u64 m = kept(j);
+        if (HOLD) tm[HOLD ? j : 0] = m;
+        s += m;
     }
     u64 all;
     u64 before = block_scan<NT, true>(s, red + 5 * NW, all);
@@ -453,8 +461,9 @@ template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sa
         int pick = -1; float pv = 0.f;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-            if (pick < 0 && r < before + tm[j]) { pick = i0 + j; pv = v[j]; }
-            before += tm[j];
+            const u64 m = HOLD ? tm[HOLD ? j : 0] : kept(j);
+            if (pick < 0 && r < before + m) { pick = i0 + j; pv = v[j]; }
+            before += m;
         }
         sample_store(a, b, pick, log_prob(w, w.at(pv), all));
     }
@@ -906,7 +915,9 @@ template <bool BF16> __global__ __launch_bounds__(512) void k_sample_draw(Sample
 }
 
 // ---- entry points -----------------------------------------------------------------------------------------------------------------------
-#define SMP_ROW_MAX (8192 - 7)          // (a row may start up to seven elements behind a 16-byte boundary)
+// (a row may start up to seven elements behind a 16-byte boundary.)  Top-k and top-p in one launch / four: 9000 tokens 20.5 / 27 us, 256 such rows 22 / 35;
+// 15000 21.7 / 28, 23 / 37; half as many in one launch 11 to 12
+#define SMP_ROW_MAX (16384 - 7)
 static int frac_bits(int V) { int c = 0; while ((1ll << c) < V) ++c; return 62 - c < 50 ? 62 - c : 50; }
 static int long_tiles(int V) { return (V + 7 + SMP_TILE - 1) / SMP_TILE; }
 // chunks of a long row: enough workgroups for the chip (1024 in all) but no more than k_sample_zone merges quickly (16, 8 KB each), at most
@@ -922,7 +933,8 @@ extern "C" size_t e2t_sample_ws_bytes(int B, int V) {
 }
 template <bool BF16> static void sample_go(SampleArgs& a, int B, void* stream) {
     if (a.V <= 2048 - 7) hipLaunchKernelGGL((k_sample_row<BF16, 256, 8>), dim3(B), dim3(256), 0, ST, a);
-    else if (a.V <= SMP_ROW_MAX) hipLaunchKernelGGL((k_sample_row<BF16, 512, 16>), dim3(B), dim3(512), 0, ST, a);
+    else if (a.V <= 8192 - 7) hipLaunchKernelGGL((k_sample_row<BF16, 512, 16>), dim3(B), dim3(512), 0, ST, a);
+    else if (a.V <= SMP_ROW_MAX) hipLaunchKernelGGL((k_sample_row<BF16, 512, 32>), dim3(B), dim3(512), 0, ST, a);
     else {
         hipLaunchKernelGGL((k_sample_hist<BF16>), dim3(a.G, B), dim3(256), 0, ST, a);
         hipLaunchKernelGGL(k_sample_zone, dim3(B), dim3(512), 0, ST, a);

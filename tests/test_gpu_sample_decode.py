@@ -10,13 +10,14 @@ from test_gpu_serving import lp_bound, product_bound, quant_oracle, sample_oracl
 
 pytestmark = pytest.mark.gpu
 EOS, PAD = 1, 0
-# a vocabulary beyond the one-launch rows: the steps share the workspace's scratch
+# vocabularies of the larger one-launch rows, and beyond them: the steps then share the workspace's scratch
 LONG = dict(channels={401: 6}, decimation=3, enc_embed=5, enc_rnn=[4, 6], dec_embed=3, dec_rnn=12, vocab=9001, aux_layer=None, ff_dropout=0.0,
             rnn_dropout=0.0)
+LONGEST = dict(LONG, vocab=20001)
 
 
 def network(name, B=19, L=6, seed=5):
-    eng, ws, ospec, P, batch = build(LONG if name == 'long' else SPECS[name], B, 26, L, seed=seed)
+    eng, ws, ospec, P, batch = build(dict(SPECS, long=LONG, longest=LONGEST)[name], B, 26, L, seed=seed)
     return eng, ws
 
 
@@ -46,7 +47,7 @@ def check_steps(eng, ws, hyp, score, u, steps, **kw):
 
 
 @pytest.mark.parametrize('int8', [False, True])
-@pytest.mark.parametrize('name', ['tiny_odd', 'small_dropout', 'cat_aux_hidden_proj', 'long'])
+@pytest.mark.parametrize('name', ['tiny_odd', 'small_dropout', 'cat_aux_hidden_proj', 'long', 'longest'])
 def test_every_step_draws_by_the_definition(name, int8):
     eng, ws = network(name)
     B, L = ws['B'], ws['L']
@@ -96,7 +97,7 @@ def test_temperature_zero_is_greedy(name):
 
 
 @pytest.mark.parametrize('int8', [False, True])
-@pytest.mark.parametrize('name', ['small_dropout', 'cat_aux_hidden_proj', 'long'])
+@pytest.mark.parametrize('name', ['small_dropout', 'cat_aux_hidden_proj', 'long', 'longest'])
 def test_one_graph_serves_all_numbers_settings_and_weights(name, int8):
     eng, ws = network(name)
     L, B = ws['L'], ws['B']

@@ -369,7 +369,7 @@ def test_sample_rows_levels_on_bin_borders(S, T, unit):
         check_sample(S, l, torch.rand(B, generator=g, device='cuda'), temperature=T, **kw)
 
 
-@pytest.mark.parametrize('V', [3, 40, 1806, 6000, 8185, 8186, 20011])
+@pytest.mark.parametrize('V', [3, 40, 1806, 2041, 2042, 6000, 8185, 8186, 16377, 16378, 20011])
 @pytest.mark.parametrize('sd,T', [(0.05, 1.0), (1e-4, 1.0), (30.0, 1.0), (1.0, 40.0), (1.0, 1e-3), (1e-30, 1.0), (1e30, 1.0)])
 def test_sample_rows_flat_and_steep(S, V, sd, T):
     """Spreads from nothing to beyond what weighs anything."""
