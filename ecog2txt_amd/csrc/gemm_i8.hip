@@ -436,34 +436,37 @@ template <int MT, int NTL, int NWV, int D> static int i8_rows_launch(const I8Arg
 // the chosen instance takes 3 % more than the best one on average and 30 % at most.  Both sides of the larger steps:
 //   M = 16, 4096 x 4096: rows 5.7, 64 x 64 tiles 14.3;   M = 128: rows 12.9, tiles in two K groups 13.0;   M = 256: rows 18.9, tiles 13.5
 //   M = 1024, 4096 x 4096: 64 x 64 39, 128 x 128 31, 128 x 128 in two K groups 26, 256 x 256 51;   M = 4096: 128 x 128 89, 256 x 256 63
-static int i8_launch(const I8Args& p, void* stream) {
-    const double S = p.S, K64 = 64.0 * S, bytes = p.N * K64;
+static int i8_instance(int M, int N, int K) {
+    const double S = (K + 63) / 64, K64 = 64.0 * S, bytes = N * K64;
     auto cdiv = [](long long a, long long b) { return (double)((a + b - 1) / b); };
     struct { double us; int kind; } best = {1e30, 0};
     auto take = [&](double us, int kind) { if (us < best.us) { best.us = us; best.kind = kind; } };
     // few rows: start and reduction, then the longest of a wave's chain of steps, the workgroups' reads (12 TB/s) and the weights' from memory
     auto rows = [&](int mt, int ntl, int nwv, double step, int kind) {
-        const double mb = cdiv(p.M, mt * 16), blocks = cdiv(p.N, ntl * 16) * mb, am = p.M < mt * 16 ? p.M : mt * 16;
+        const double mb = cdiv(M, mt * 16), blocks = cdiv(N, ntl * 16) * mb, am = M < mt * 16 ? M : mt * 16;
         const double l2 = blocks * (am + ntl * 16) * K64 / 1.2e7, mem = bytes / 5e6 * (bytes > 3e7 ? mb : 1);
         take(2.2 + 0.5 * mt * ntl + (nwv == 8 ? 0.2 : 0) + fmax(fmax(l2, mem), S / nwv * step), kind);
     };
-    if (p.M <= 512) {
+    if (M <= 512) {
         rows(1, 1, 4, 0.125, 0); rows(1, 1, 8, 0.144, 1); rows(1, 2, 4, 0.14, 2); rows(2, 1, 4, 0.14, 3); rows(2, 2, 4, 0.16, 4); rows(2, 4, 4, 0.18, 5);
     }
     // tiles: the latency of one tile, or the chip's throughput where they queue up
     auto tiles = [&](int t, double step, double fill, double per_step, double per_tile, double base, int kind) {
-        const double W = cdiv(p.M, t) * cdiv(p.N, t), even = W + 0.66 * (256.0 * ceil(W / 256) - W);      // (some CUs have a tile more than others)
+        const double W = cdiv(M, t) * cdiv(N, t), even = W + 0.66 * (256.0 * ceil(W / 256) - W);      // (some CUs have a tile more than others)
         take(fmax(fmax(step * S + fill, per_step * even * S + per_tile * W + base), 2.7 + bytes / 5e6), kind);
         return W;
     };
     if (tiles(64, 0.20, 4.2, 0.0006, 0.0012, 4.0, 6) <= 256) take(fmax(0.13 * S + 5.0, 2.7 + bytes / 5e6), 7);
     if (tiles(128, 0.36, 7.5, 0.0011, 0.0064, 5.0, 8) <= 256) take(fmax(0.27 * S + 8.5, 2.7 + bytes / 5e6), 9);
     {
-        const double W = cdiv(p.M, 256) * cdiv(p.N, 256), left = W < 256 ? 0 : W - 256 * floor(W / 256);
+        const double W = cdiv(M, 256) * cdiv(N, 256), left = W < 256 ? 0 : W - 256 * floor(W / 256);
         const double round = W < 256 ? 0.7 * S + 11 : 0.85 * S + 13;
         take((W < 256 ? 1 : floor(W / 256)) * round + (left == 0 ? 0 : left <= I8_QUARTERED ? 0.27 * round : round), 10);
     }
-    switch (best.kind) {
+    return best.kind;
+}
+static int i8_launch(const I8Args& p, void* stream) {
+    switch (i8_instance(p.M, p.N, p.K)) {
     case 0: return i8_rows_launch<1, 1, 4, 4>(p, stream);
     case 1: return i8_rows_launch<1, 1, 8, 4>(p, stream);
     case 2: return i8_rows_launch<1, 2, 4, 4>(p, stream);
@@ -526,6 +529,10 @@ extern "C" int e2t_gemm_nt_i8(const int8_t* A, long long lda, const float* sa, c
     I8Args p = i8_args(B, ldb, sb, bias, C, ldc, M, N, K, flags);
     p.A = A; p.sa = sa; p.lda = lda;
     return i8_launch(p, stream);
+}
+
+extern "C" int e2t_gemm_i8_instance(int M, int N, int K) {
+    return M > 0 && M <= E2T_I8_MAX_ROWS && N > 0 && N <= E2T_I8_MAX_ROWS && K > 0 && K <= E2T_I8_MAX_K ? i8_instance(M, N, K) : -1;
 }
 
 static inline size_t lin_q_bytes(int M, int K) { return ((size_t)M * (size_t)((K + 63) & ~63) + 255) & ~(size_t)255; }

@@ -145,7 +145,7 @@ SIGNATURES = {
 COMM_ID_BYTES = 128
 PLAIN = {'e2t_abi_version': ([], C.c_int), 'e2t_sizeof': ([_i], C.c_int), 'e2t_last_error': ([], C.c_char_p), 'e2t_device_cus': ([_i], C.c_int),
          'e2t_bwd_persist_kq': ([_i], C.c_int), 'e2t_lstm_big_ok': ([_i], C.c_int), 'e2t_conv_fwd_fused_ok': ([_i, _i], C.c_int), 'e2t_comm_rank': ([_p], C.c_int), 'e2t_comm_size': ([_p], C.c_int),
-         'e2t_linear_i8_ws_bytes': ([_i, _i, _i], C.c_size_t), 'e2t_sample_ws_bytes': ([_i, _i], C.c_size_t),
+         'e2t_gemm_i8_instance': ([_i, _i, _i], C.c_int), 'e2t_linear_i8_ws_bytes': ([_i, _i, _i], C.c_size_t), 'e2t_sample_ws_bytes': ([_i, _i], C.c_size_t),
          'e2t_crc32c': ([_p, _z, C.c_uint32], C.c_uint32)}
 
 _lib = None

@@ -338,6 +338,9 @@ int e2t_quant_rows_i8(const void* x, int dtype, long long ldx, int M, int K, int
 #define E2T_I8_MAX_LD 8388608       /* largest lda / ldb: a tile's rows are addressed with 32 bits */
 int e2t_gemm_nt_i8(const int8_t* A, long long lda, const float* sa, const int8_t* B, long long ldb, const float* sb, const float* bias,
                    void* C, long long ldc, int M, int N, int K, int flags, void* stream);
+/* which of the product's instances these sizes run on, 0 .. 10 (-1: sizes that are refused): the sums are the same on all of them; for
+ * tests, which have to reach each */
+int e2t_gemm_i8_instance(int M, int N, int K);
 /* the same from activations: e2t_quant_rows_i8(x) and e2t_gemm_nt_i8 in one call.  ws: device memory of e2t_linear_i8_ws_bytes(M, N, K),
  * 16-B aligned, needed until the call has run; its content does not matter.  (0 where none is needed: ws may then be NULL.) */
 size_t e2t_linear_i8_ws_bytes(int M, int N, int K);
