@@ -10,6 +10,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/object_ptr.h>
 #include "ecog2txt_hip.h"
 
 namespace {
@@ -17,7 +18,7 @@ namespace {
 #define X(f) decltype(&::f) f##_p = nullptr;
 E2T_BOUND(X)
 #undef X
-PyObject *raw_stream, *s_q, *s_scale, *s_cols, *s_ld, *rows_type;        // torch's current-stream function; attribute names and class of Int8Rows
+PyObject *raw_stream, *s_q, *s_scale, *s_cols, *rows_type;        // torch's current-stream function; attribute names and class of Int8Rows
 
 struct Bad {};                                             // (the Python error is set)
 [[noreturn]] void bad(const char* f, ...) {
@@ -77,29 +78,38 @@ template <class F, class... A> void call(const char* name, int dev, F f, A... a)
     if (rc) { PyErr_Format(PyExc_RuntimeError, "%s failed (%d): %s", name, rc, e2t_last_error_p()); throw Bad(); }
 }
 
-// an Int8Rows, by its attributes
+// q and scale of a matrix in 8 bits with `cols` columns: its row stride
+int64_t rows_stride(PyObject* q, PyObject* scale, int64_t cols) {
+    Mat m = matrix(q, "q", at::kChar, at::kChar);
+    if (cols <= 0 || cols > E2T_I8_MAX_ROWS || (cols + 63) / 64 * 64 > m.cols)
+        bad("q needs %lld columns (the %lld of the matrix, rounded up to 64)", (long long)(cols + 63) / 64 * 64, (long long)cols);
+    if (cols > E2T_I8_MAX_K) bad("more than %d columns overflow the 32-bit sums", E2T_I8_MAX_K);
+    if (m.rows <= 1) m.ld = m.cols / 64 * 64;
+    if (((uintptr_t)m.t->data_ptr() | (uintptr_t)m.ld) & 15) bad("the rows of q must start on 16-byte boundaries");
+    vector(scale, m.rows, at::kFloat, m.dev, "scale");
+    return m.ld;
+}
+// an Int8Rows, by its attributes, which may have been set (or their tensors resized) since it was made: they are checked in every call
 struct Rows {
-    PyObject *q = nullptr, *scale = nullptr;
+    THPObjectPtr q, scale;
     int64_t cols = 0, ld = 0;
     explicit Rows(PyObject* o, const char* name) {
         const int is = PyObject_IsInstance(o, rows_type);
         if (is < 0) throw Bad();
         if (!is) bad("%s must be Int8Rows", name);
-        PyObject *c = PyObject_GetAttr(o, s_cols), *l = PyObject_GetAttr(o, s_ld);
+        THPObjectPtr c(PyObject_GetAttr(o, s_cols));
         q = PyObject_GetAttr(o, s_q); scale = PyObject_GetAttr(o, s_scale);
-        const bool ok = c && l && q && scale && THPVariable_Check(q) && THPVariable_Check(scale);
-        if (ok) { cols = PyLong_AsLongLong(c); ld = PyLong_AsLongLong(l); }
-        Py_XDECREF(c); Py_XDECREF(l);
-        if (!ok || PyErr_Occurred()) { Py_XDECREF(q); Py_XDECREF(scale); if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "ecog2txt_amd.serving: broken Int8Rows"); throw Bad(); }
+        if (!c || !q || !scale) throw Bad();
+        cols = PyLong_AsLongLong(c.get());
+        if (cols == -1 && PyErr_Occurred()) throw Bad();
+        ld = rows_stride(q.get(), scale.get(), cols);
     }
-    ~Rows() { Py_XDECREF(q); Py_XDECREF(scale); }
-    Rows(const Rows&) = delete;
-    const at::Tensor& qt() const { return THPVariable_Unpack(q); }
-    const float* sp() const { return (const float*)THPVariable_Unpack(scale).data_ptr(); }
+    const at::Tensor& qt() { return THPVariable_Unpack(q.get()); }
+    const float* sp() { return (const float*)THPVariable_Unpack(scale.get()).data_ptr(); }
 };
 struct Out { at::Tensor made; const at::Tensor* t; int64_t n, ld; const float* bias; int flags; };
 // weights, bias, output type and output of a product with `rows` rows of activations
-Out output(const Rows& w, int64_t cols, PyObject* bias, PyObject* out_dtype, PyObject* relu, PyObject* out, int64_t rows, const at::Tensor& like) {
+Out output(Rows& w, int64_t cols, PyObject* bias, PyObject* out_dtype, PyObject* relu, PyObject* out, int64_t rows, const at::Tensor& like) {
     const int dev = like.get_device();
     if (w.qt().get_device() != dev) bad("the weights must be Int8Rows on device %d", dev);
     if (w.cols != cols) bad("%lld columns of activations, %lld of weights", (long long)cols, (long long)w.cols);
@@ -136,16 +146,9 @@ PyObject* bind(PyObject*, PyObject* const*, Py_ssize_t);
 
 // check_rows(q, scale, cols) -> row stride
 E2T_PY(check_rows, 3) {
-    Mat m = matrix(a[0], "q", at::kChar, at::kChar);
     const int64_t cols = PyLong_AsLongLong(a[2]);
     if (cols == -1 && PyErr_Occurred()) throw Bad();
-    if (cols <= 0 || cols > E2T_I8_MAX_ROWS || (cols + 63) / 64 * 64 > m.cols)
-        bad("q needs %lld columns (the %lld of the matrix, rounded up to 64)", (long long)(cols + 63) / 64 * 64, (long long)cols);
-    if (cols > E2T_I8_MAX_K) bad("more than %d columns overflow the 32-bit sums", E2T_I8_MAX_K);
-    if (m.rows <= 1) m.ld = m.cols / 64 * 64;
-    if (((uintptr_t)m.t->data_ptr() | (uintptr_t)m.ld) & 15) bad("the rows of q must start on 16-byte boundaries");
-    vector(a[1], m.rows, at::kFloat, m.dev, "scale");
-    return PyLong_FromLongLong(m.ld);
+    return PyLong_FromLongLong(rows_stride(a[0], a[1], cols));
 }
 // quantize(x) -> q, scale
 E2T_PY(quantize, 1) {
@@ -158,7 +161,7 @@ E2T_PY(quantize, 1) {
 }
 // matmul(a, w, bias, out_dtype, relu, out) -> out
 E2T_PY(matmul, 6) {
-    const Rows x(a[0], "a"), w(a[1], "w");
+    Rows x(a[0], "a"), w(a[1], "w");
     const at::Tensor& q = x.qt();
     const Out o = output(w, x.cols, a[2], a[3], a[4], a[5], q.size(0), q);
     if (q.size(0))
@@ -169,7 +172,7 @@ E2T_PY(matmul, 6) {
 // linear(x, w, bias, out_dtype, relu, out) -> out
 E2T_PY(linear, 6) {
     const Mat x = matrix(a[0], "x", at::kFloat, at::kBFloat16);
-    const Rows w(a[1], "w");
+    Rows w(a[1], "w");
     const Out o = output(w, x.cols, a[2], a[3], a[4], a[5], x.rows, *x.t);
     if (x.rows) {
         const size_t need = e2t_linear_i8_ws_bytes_p((int)x.rows, (int)o.n, (int)x.cols);
@@ -233,6 +236,6 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_serving_host", nullptr, -1, metho
 
 PyMODINIT_FUNC PyInit__serving_host() {
     s_q = PyUnicode_InternFromString("q"); s_scale = PyUnicode_InternFromString("scale");
-    s_cols = PyUnicode_InternFromString("cols"); s_ld = PyUnicode_InternFromString("ld");
-    return s_q && s_scale && s_cols && s_ld ? PyModule_Create(&module) : nullptr;
+    s_cols = PyUnicode_InternFromString("cols");
+    return s_q && s_scale && s_cols ? PyModule_Create(&module) : nullptr;
 }
