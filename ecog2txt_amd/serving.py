@@ -4,7 +4,7 @@ tensors' device.  Workspaces come from torch's allocator per call, so calls on d
 share none.  Weights are quantised once (`quantize_rows`) and kept by the caller as an `Int8Rows`.
 
 The checks and the calls themselves are native (csrc/serving_host.cpp).  What cannot be served raises ValueError; nothing here has a
-gradient: tensors that ask for one are refused."""
+gradient: tensors that ask for one, operands, scales, bias and settings alike, are refused, in forward mode too."""
 import ctypes as C
 
 import torch
@@ -66,6 +66,8 @@ def linear_i8(x, w, bias=None, out_dtype=torch.float32, relu=False, out=None):
 
 
 def _rows_array(v, rows, dtype, index, name):
+    if v.requires_grad and torch.is_grad_enabled():
+        raise ValueError('ecog2txt_amd.serving: %s asks for a gradient: the serving operators have none (use torch.no_grad())' % name)
     if v.dtype is not dtype or v.get_device() != index or v.dim() != 1 or v.shape[0] != rows or not v.is_contiguous():
         raise ValueError('ecog2txt_amd.serving: %s must be a contiguous %s tensor of %d on device %d' % (name, str(dtype).replace('torch.', ''), rows, index))
     return v.data_ptr()

@@ -50,3 +50,32 @@ def test_rows_in_8_bits_are_checked_in_every_call(S):
     wide[:, :128] = w.q
     w.q = wide                                                         # (another row stride)
     assert torch.equal(S.matmul_i8(a, w), want[2:5])
+
+
+def test_gradients_are_refused_not_lost(S):
+    """Every tensor a call takes, asking for a gradient in either mode; without gradients the same calls pass."""
+    import torch.autograd.forward_ad as fw
+    x, weight = torch.randn(3, 100, generator=gen(1), device='cuda'), torch.randn(50, 100, generator=gen(2), device='cuda')
+    a, w = S.quantize_rows(x), S.quantize_rows(weight)
+    ones = lambda *n: torch.ones(*n, device='cuda')
+    calls = [lambda g: S.quantize_rows(g(x)), lambda g: S.linear_i8(g(x), w), lambda g: S.linear_i8(x, w, bias=g(ones(50))), lambda g: S.matmul_i8(a, w, bias=g(ones(50))),
+             lambda g: S.matmul_i8(a, w, out=g(ones(3, 50))), lambda g: S.linear_i8(x, w, out=g(ones(3, 50))), lambda g: S.Int8Rows(w.q, g(ones(50)), 100),
+             lambda g: S.sample_rows(g(x), ones(3) / 2), lambda g: S.sample_rows(x, g(ones(3) / 2)), lambda g: S.sample_rows(x, ones(3) / 2, temperature=g(ones(3))),
+             lambda g: S.sample_rows(x, ones(3) / 2, top_p=g(ones(3))), lambda g: S.sample_rows(x, ones(3) / 2, min_p=g(ones(3))),
+             lambda g: S.sample_config(3, x.get_device(), temperature=g(ones(3)))]
+    for c in calls:
+        with pytest.raises(ValueError, match='gradient'):
+            c(lambda t: t.clone().requires_grad_())
+        with pytest.raises(ValueError, match='gradient'):
+            c(lambda t: t.clone().requires_grad_() * 1)
+        c(lambda t: t)
+        with torch.no_grad():
+            c(lambda t: t.clone().requires_grad_())
+    for c in calls[:-1]:
+        with fw.dual_level():
+            with pytest.raises(ValueError, match='tangent'):
+                c(lambda t: fw.make_dual(t.clone(), torch.ones_like(t)))
+    with torch.no_grad():                                              # scales learned elsewhere, used with gradients on
+        r = S.Int8Rows(w.q, ones(50).requires_grad_(), 100)
+    with pytest.raises(ValueError, match='gradient'):
+        S.linear_i8(x, r)

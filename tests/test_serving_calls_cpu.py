@@ -1,0 +1,17 @@
+"""What the tensor-level serving calls refuse whatever device a tensor lies on (no GPU needed)."""
+import pytest
+import torch
+
+
+def test_gradients():
+    import torch.autograd.forward_ad as fw
+    from ecog2txt_amd import serving as S
+    x = torch.zeros(3, 64)
+    with pytest.raises(ValueError, match='gradient'):
+        S.quantize_rows(x.clone().requires_grad_())
+    with pytest.raises(ValueError, match='gradient'):
+        S.sample_config(3, -1, top_p=torch.ones(3).requires_grad_())
+    with fw.dual_level(), pytest.raises(ValueError, match='tangent'):
+        S.linear_i8(fw.make_dual(x, x + 1), None)
+    with torch.no_grad(), pytest.raises(ValueError, match='device tensor'):
+        S.quantize_rows(x.clone().requires_grad_())
