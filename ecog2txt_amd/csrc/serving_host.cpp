@@ -136,7 +136,12 @@ Out output(Rows& w, int64_t cols, PyObject* bias, PyObject* out_dtype, PyObject*
     return o;
 }
 int dt_of(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 ? E2T_DT_BF16 : E2T_DT_F32; }
-PyObject* wrap(const Out& o, PyObject* out) { if (out != Py_None) { Py_INCREF(out); return out; } return THPVariable_Wrap(o.made); }
+PyObject* wrap(const Out& o, PyObject* out) {
+    if (out == Py_None) return THPVariable_Wrap(o.made);
+    if (!o.t->is_inference()) o.t->unsafeGetTensorImpl()->bump_version();       // (a graph that saved its old values notices)
+    Py_INCREF(out);
+    return out;
+}
 
 PyObject* bind(PyObject*, PyObject* const*, Py_ssize_t);
 // every entry: C++ exceptions become Python's

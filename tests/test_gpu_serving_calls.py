@@ -79,3 +79,18 @@ def test_gradients_are_refused_not_lost(S):
         r = S.Int8Rows(w.q, ones(50).requires_grad_(), 100)
     with pytest.raises(ValueError, match='gradient'):
         S.linear_i8(x, r)
+
+
+def test_writing_out_is_noticed_by_graphs_that_saved_it(S):
+    x, w = torch.randn(3, 100, generator=gen(1), device='cuda'), S.quantize_rows(torch.randn(50, 100, generator=gen(2), device='cuda'))
+    for write in (lambda out: S.linear_i8(x, w, out=out), lambda out: S.matmul_i8(S.quantize_rows(x), w, out=out)):
+        out = torch.ones(5, 50, device='cuda')
+        v = torch.ones(5, 50, device='cuda', requires_grad=True)
+        loss = (v * out).sum()
+        write(out[1:4])                                                # (a view: the counter is its base's)
+        with pytest.raises(RuntimeError, match='inplace'):
+            loss.backward()
+        with torch.inference_mode():
+            o = torch.ones(3, 50, device='cuda')
+            assert write(o) is o
+        assert torch.equal(write(o), write(None))
