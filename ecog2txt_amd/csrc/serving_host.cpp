@@ -33,17 +33,19 @@ struct Bad {};                                             // (the Python error 
 }
 const char* type_name(at::ScalarType t) { return t == at::kFloat ? "float32" : t == at::kInt ? "int32" : t == at::kChar ? "int8" : "bfloat16"; }
 
-// nothing here has a gradient: a tensor that asks for one, in reverse or in forward mode, is refused
-void no_gradient(const at::Tensor& t, const char* name) {
+// nothing here has a gradient: a tensor that asks for one, in reverse or in forward mode, is refused; and memory is read as it lies, so
+// that a view which stands for its negative (the imaginary part of a conjugate) is refused, too
+void plain(const at::Tensor& t, const char* name) {
     if (t.requires_grad() && at::GradMode::is_enabled()) bad("%s asks for a gradient: the serving operators have none (use torch.no_grad())", name);
     if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
         bad("%s has a forward-mode tangent: the serving operators pass none on", name);
+    if (t.is_neg()) bad("%s is a view of the negative of what its memory holds (use its resolve_neg())", name);
 }
 struct Mat { const at::Tensor* t; int64_t rows, cols, ld; int dev; };
 // a 2-D device tensor with contiguous rows
 Mat matrix(PyObject* o, const char* name, at::ScalarType t0, at::ScalarType t1) {
     const bool is = THPVariable_Check(o);
-    if (is) no_gradient(THPVariable_Unpack(o), name);
+    if (is) plain(THPVariable_Unpack(o), name);
     if (!is || !THPVariable_Unpack(o).is_cuda() || THPVariable_Unpack(o).dim() != 2 || (THPVariable_Unpack(o).scalar_type() != t0 && THPVariable_Unpack(o).scalar_type() != t1))
         bad("%s must be a 2-D device tensor of %s%s%s", name, type_name(t0), t0 != t1 ? " / " : "", t0 != t1 ? type_name(t1) : "");
     const at::Tensor& t = THPVariable_Unpack(o);
@@ -57,7 +59,7 @@ Mat matrix(PyObject* o, const char* name, at::ScalarType t0, at::ScalarType t1) 
 void* vector(PyObject* o, int64_t n, at::ScalarType type, int dev, const char* name) {
     if (THPVariable_Check(o)) {
         const at::Tensor& t = THPVariable_Unpack(o);
-        no_gradient(t, name);
+        plain(t, name);
         if (t.scalar_type() == type && t.is_cuda() && t.get_device() == dev && t.dim() == 1 && t.size(0) == n && t.is_contiguous()) return t.data_ptr();
     }
     bad("%s must be a contiguous %s tensor of %lld on device %d", name, type_name(type), (long long)n, dev);

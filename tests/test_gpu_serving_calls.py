@@ -94,3 +94,18 @@ def test_writing_out_is_noticed_by_graphs_that_saved_it(S):
             o = torch.ones(3, 50, device='cuda')
             assert write(o) is o
         assert torch.equal(write(o), write(None))
+
+
+def test_negated_views(S):
+    """The imaginary part of a conjugate is a view whose memory holds the opposite sign."""
+    z = torch.randn(4, 1, dtype=torch.complex64, generator=gen(1), device='cuda')
+    x, one = z.conj().imag, z[:1, 0].conj().imag
+    assert x.is_neg() and one.is_neg()
+    w = S.quantize_rows(torch.ones(1, 1, device='cuda'))
+    for call in (lambda f: S.quantize_rows(f(x)), lambda f: S.linear_i8(f(x), w), lambda f: S.linear_i8(x.resolve_neg(), w, bias=f(one)),
+                 lambda f: S.sample_rows(f(x), torch.zeros(4, device='cuda')), lambda f: S.sample_rows(x.resolve_neg()[:1], f(one))):
+        with pytest.raises(ValueError, match='resolve_neg'):
+            call(lambda t: t)
+        call(lambda t: t.resolve_neg())
+    r = S.quantize_rows(x.resolve_neg()).float()
+    assert torch.equal(r.sign(), -z.imag.sign())

@@ -15,3 +15,11 @@ def test_gradients():
         S.linear_i8(fw.make_dual(x, x + 1), None)
     with torch.no_grad(), pytest.raises(ValueError, match='device tensor'):
         S.quantize_rows(x.clone().requires_grad_())
+
+
+def test_negated_views():
+    from ecog2txt_amd import serving as S
+    x = torch.zeros(3, 1, dtype=torch.complex64).conj().imag
+    assert x.is_neg()
+    with pytest.raises(ValueError, match='resolve_neg'):
+        S.quantize_rows(x)
