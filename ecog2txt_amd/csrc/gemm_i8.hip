@@ -98,7 +98,7 @@ struct I8Args {
 };
 __device__ __forceinline__ float i8_scale(int acc, float sa, float sb, float bias, int relu) {
     float y = (float)acc * sa * sb + bias;
-    return relu ? fmaxf(y, 0.f) : y;
+    return relu && y < 0.f ? 0.f : y;                      // (fmaxf would turn a NaN of a scale or bias into 0)
 }
 // ---- tiled product -----------------------------------------------------------------------------------------------------------------
 // BM x BN tile, WM x WN waves, v_mfma_i32_16x16x64_i8 (16 B of k a lane: operands lie in memory as the instruction wants them).

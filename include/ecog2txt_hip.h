@@ -331,7 +331,7 @@ int e2t_quant_rows_i8(const void* x, int dtype, long long ldx, int M, int K, int
 /* C[m][n] = sa[m] * sb[n] * sum_k A[m][k] * B[n][k] (+ bias[n]): A int8 [M][lda] (one scale a row = token), B int8 [N][ldb] (one scale a
  * row = output channel), both 16-B aligned with leading dimensions that are multiples of 16 and >= K rounded up to 64; columns
  * from K up to that must be zero in at least one of the two (e2t_quant_rows_i8 writes them so).  The integer sum is exact
- * (K <= E2T_I8_MAX_K), then rounded to fp32 once and multiplied by sa, then by sb; bias and the optional ReLU in fp32.  flags:
+ * (K <= E2T_I8_MAX_K), then rounded to fp32 once and multiplied by sa, then by sb; bias and the optional ReLU (which leaves a NaN one) in fp32.  flags:
  * E2T_GEMM_RELU, E2T_GEMM_OUT_BF16 (C bf16 instead of fp32); others are refused.  C overlaps none of the inputs. */
 #define E2T_I8_MAX_ROWS (1 << 30)   /* M, N */
 #define E2T_I8_MAX_K 131071

@@ -109,3 +109,17 @@ def test_negated_views(S):
         call(lambda t: t.resolve_neg())
     r = S.quantize_rows(x.resolve_neg()).float()
     assert torch.equal(r.sign(), -z.imag.sign())
+
+
+@pytest.mark.parametrize('M,N,K', [(1, 50, 100), (7, 300, 640), (700, 300, 64), (2049, 2310, 200), (1942, 1765, 910), (1624, 4899, 144)])
+def test_relu_keeps_nan(S, M, N, K):
+    """NaN from a bias or a scale stays NaN behind the ReLU, on few rows, tiles and the fused layer."""
+    x = torch.randn(M, K, generator=gen(1), device='cuda')
+    a, w = S.quantize_rows(x), S.quantize_rows(torch.randn(N, K, generator=gen(2), device='cuda'))
+    bias = torch.randn(N, generator=gen(3), device='cuda')
+    bias[3] = float('nan'); w.scale[5] = float('nan'); bias[7] = float('-inf'); bias[8] = float('inf')
+    for out in (torch.float32, torch.bfloat16):
+        for f in (lambda **kw: S.matmul_i8(a, w, bias=bias, out_dtype=out, **kw), lambda **kw: S.linear_i8(x, w, bias=bias, out_dtype=out, **kw)):
+            y, r = f(), f(relu=True)
+            assert torch.equal(y.isnan().any(0).nonzero()[:, 0], torch.tensor([3, 5], device='cuda')) and y[:, [3, 5]].isnan().all()
+            assert torch.equal(r.isnan(), y.isnan()) and torch.equal(r.nan_to_num(nan=1.0), torch.relu(y).nan_to_num(nan=1.0))
