@@ -391,8 +391,9 @@ __global__ __launch_bounds__(64 * NWV) void k_gemm_i8_rows(I8Args p) {
     for (int e = tid; e < MR * NC; e += NT) {
         const int ml = e / NC, c = n0 + (e - ml * NC), m = m0 + ml;
         if (m >= p.M || c >= p.N) continue;
+        // (f2bf_pk: a NaN stays one whatever its low bits; f2bf's addition carries them into the sign)
         const float y = i8_scale(part[e], FUSED ? sxs[ml] : p.sa[m], p.sb[c], p.bias ? p.bias[c] : 0.f, p.relu);
-        if (p.out_bf16) ((bf16_t*)p.C)[(size_t)m * p.ldc + c] = f2bf(y); else ((float*)p.C)[(size_t)m * p.ldc + c] = y;
+        if (p.out_bf16) ((bf16_t*)p.C)[(size_t)m * p.ldc + c] = (bf16_t)f2bf_pk(y, y); else ((float*)p.C)[(size_t)m * p.ldc + c] = y;
     }
 }
 

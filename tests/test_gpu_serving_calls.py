@@ -123,3 +123,15 @@ def test_relu_keeps_nan(S, M, N, K):
             y, r = f(), f(relu=True)
             assert torch.equal(y.isnan().any(0).nonzero()[:, 0], torch.tensor([3, 5], device='cuda')) and y[:, [3, 5]].isnan().all()
             assert torch.equal(r.isnan(), y.isnan()) and torch.equal(r.nan_to_num(nan=1.0), torch.relu(y).nan_to_num(nan=1.0))
+
+
+@pytest.mark.parametrize('bits', [-1, 0x7FFFFFFF, 0x7FC00000, 0x7F800001, -0x400000])
+@pytest.mark.parametrize('M,N,K', [(1, 50, 100), (16, 50, 640), (700, 300, 64)])
+def test_nan_of_any_payload_in_bf16_outputs(S, M, N, K, bits):
+    """A NaN whose low bits are ones would round up past the largest exponent as a number would."""
+    x = torch.randn(M, K, generator=gen(1), device='cuda')
+    a, w = S.quantize_rows(x), S.quantize_rows(torch.randn(N, K, generator=gen(2), device='cuda'))
+    bias = torch.zeros(N, device='cuda')
+    bias.view(torch.int32)[3] = bits
+    for y in (S.matmul_i8(a, w, bias=bias, out_dtype=torch.bfloat16), S.linear_i8(x, w, bias=bias, out_dtype=torch.bfloat16)):
+        assert torch.equal(y.isnan().any(0).nonzero()[:, 0], torch.tensor([3], device='cuda')) and y[:, 3].isnan().all()
