@@ -928,8 +928,13 @@ static int long_chunks(int B, int V) {
     if (want > 16) want = 16;
     return want < least ? least : want > tiles ? tiles : want;
 }
+// rows of one launch: in grid.y for long rows, in grid.x (below 2^32 threads) for others; larger batches run in pieces, one behind the other in the
+// same workspace
+static int rows_a_launch(int B, int V) { const int most = V > SMP_ROW_MAX ? 65535 : 1 << 22; return B < most ? B : most; }
 extern "C" size_t e2t_sample_ws_bytes(int B, int V) {
-    return B > 0 && V > SMP_ROW_MAX && V <= E2T_SAMPLE_MAX_V ? (size_t)B * row_ws_bytes(long_chunks(B, V), long_tiles(V)) : 0;
+    if (B <= 0 || V <= SMP_ROW_MAX || V > E2T_SAMPLE_MAX_V) return 0;
+    const int n = rows_a_launch(B, V);
+    return (size_t)n * row_ws_bytes(long_chunks(n, V), long_tiles(V));
 }
 template <bool BF16> static void sample_go(SampleArgs& a, int B, void* stream) {
     if (a.V <= 2048 - 7) hipLaunchKernelGGL((k_sample_row<BF16, 256, 8>), dim3(B), dim3(256), 0, ST, a);
@@ -943,7 +948,7 @@ template <bool BF16> static void sample_go(SampleArgs& a, int B, void* stream) {
     }
 }
 static int sample_launch(SampleArgs& a, int dtype, int B, const e2t_sample_cfg* cfg, void* ws, size_t ws_bytes, void* stream) {
-    E2T_CHECK_ARG(a.logits && a.u && cfg && B > 0 && B <= 65535 && a.V > 0 && a.V <= E2T_SAMPLE_MAX_V && a.ldl >= a.V);
+    E2T_CHECK_ARG(a.logits && a.u && cfg && B > 0 && a.V > 0 && a.V <= E2T_SAMPLE_MAX_V && a.ldl >= a.V);
     E2T_CHECK_ARG(dtype == E2T_DT_F32 || dtype == E2T_DT_BF16);
     E2T_CHECK_ARG(((uintptr_t)a.logits & (dtype == E2T_DT_F32 ? 3 : 1)) == 0);
     const size_t need = e2t_sample_ws_bytes(B, a.V);
@@ -951,9 +956,19 @@ static int sample_launch(SampleArgs& a, int dtype, int B, const e2t_sample_cfg* 
     a.frac = frac_bits(a.V);
     a.t0 = cfg->temperature; a.k0 = cfg->top_k; a.p0 = cfg->top_p; a.m0 = cfg->min_p;
     a.t = cfg->temperature_rows; a.k = cfg->top_k_rows; a.p = cfg->top_p_rows; a.m = cfg->min_p_rows;
-    a.ws = (char*)ws; a.G = long_chunks(B, a.V); a.tiles = long_tiles(a.V);
-    if (dtype == E2T_DT_BF16) sample_go<true>(a, B, stream); else sample_go<false>(a, B, stream);
-    E2T_LAUNCH_CHECK(); return E2T_OK;
+    const int n = rows_a_launch(B, a.V);
+    a.ws = (char*)ws; a.G = long_chunks(n, a.V); a.tiles = long_tiles(a.V);
+    for (long long b0 = 0; b0 < B; b0 += n) {
+        SampleArgs s = a;
+        auto from = [&](auto*& p, long long step) { if (p) p += b0 * step; };
+        s.logits = (const char*)a.logits + (size_t)b0 * a.ldl * (dtype == E2T_DT_BF16 ? 2 : 4);
+        from(s.u, 1); from(s.t, 1); from(s.k, 1); from(s.p, 1); from(s.m, 1); from(s.token, 1); from(s.logprob, 1);
+        from(s.done, 1); from(s.out, a.Lmax); from(s.next_tok, 1); from(s.score, 1);
+        const int rows = (int)(B - b0 < n ? B - b0 : n);
+        if (dtype == E2T_DT_BF16) sample_go<true>(s, rows, stream); else sample_go<false>(s, rows, stream);
+        E2T_LAUNCH_CHECK();
+    }
+    return E2T_OK;
 }
 extern "C" int e2t_sample_rows(const void* logits, int dtype, long long ldl, int B, int V, const float* u, const e2t_sample_cfg* cfg,
                                int32_t* token, float* logprob, void* ws, size_t ws_bytes, void* stream) {

@@ -355,7 +355,7 @@ int e2t_linear_i8(const void* x, int dtype, long long ldx, const int8_t* W, long
  * token's probability among the kept ones (0 for temperature <= 0, -inf for token -1).
  * Sums are of whole numbers (probabilities in units of 2^-F of the largest, F = min(50, 62 - ceil(log2 V)), each good to 2e-14 of its
  * value or half a unit), so the answer does not depend on their order; what lies 32 or more below the largest z weighs nothing.
- * In rows above 16377 tokens the sum that top_p is a share of is good to 1e-11 only, in a way that depends on B.  A settings array, where given, holds one value a row (device memory);
+ * In rows above 16377 tokens the sum that top_p is a share of is good to 1e-11 only, in a way that depends on B.  Any number of rows; V at most E2T_SAMPLE_MAX_V.  A settings array, where given, holds one value a row (device memory);
  * the scalar counts where it is NULL.  ws: device memory of e2t_sample_ws_bytes(B, V), 16-B aligned, needed until the call has run. */
 #define E2T_SAMPLE_MAX_V 1048576
 typedef struct e2t_sample_cfg {

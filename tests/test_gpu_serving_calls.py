@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_serving import gen
+from test_gpu_serving import check_sample, gen
 
 pytestmark = pytest.mark.gpu
 
@@ -135,3 +135,60 @@ def test_nan_of_any_payload_in_bf16_outputs(S, M, N, K, bits):
     bias.view(torch.int32)[3] = bits
     for y in (S.matmul_i8(a, w, bias=bias, out_dtype=torch.bfloat16), S.linear_i8(x, w, bias=bias, out_dtype=torch.bfloat16)):
         assert torch.equal(y.isnan().any(0).nonzero()[:, 0], torch.tensor([3], device='cuda')) and y[:, 3].isnan().all()
+
+
+def settings(B, seed):
+    r = torch.rand(4, B, generator=gen(seed), device='cuda')
+    return dict(temperature=0.5 + r[0], top_k=(r[1] * 40).int(), top_p=0.5 + r[2], min_p=0.1 * r[3])
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('B,V', [(65535, 70), (65536, 70), (70001, 1806), ((1 << 22) + 5, 3)])
+def test_sample_rows_of_any_number(S, B, V, dtype):
+    l = (torch.randn(B, V, generator=gen(B), device='cuda') * 2).to(dtype)
+    u, kw = torch.rand(B, generator=gen(2), device='cuda'), settings(B, 3)
+    tok, lp = S.sample_rows(l, u, **kw)
+    for a in range(0, B, 60000 if B < 1 << 20 else 3 << 20):
+        z = min(B, a + (60000 if B < 1 << 20 else 3 << 20))
+        t, p = S.sample_rows(l[a:z], u[a:z], **{n: v[a:z] for n, v in kw.items()})
+        assert torch.equal(t, tok[a:z]) and torch.equal(p, lp[a:z])
+    check_sample(S, l[-40:], u[-40:], **{n: v[-40:] for n, v in kw.items()})
+
+
+def test_sample_long_rows_of_any_number(S):
+    """More long rows than a launch has: copies of a few, each like its original (top-p apart, whose sums depend on the split)."""
+    B, V, n = 65535 + 700, 16378, 37
+    few, u = (torch.randn(n, V, generator=gen(1), device='cuda') * 2).bfloat16(), torch.rand(n, generator=gen(2), device='cuda')
+    kw = dict(settings(n, 3), top_p=1.0)
+    i = torch.arange(B, device='cuda') % n
+    big = {k: v[i] if isinstance(v, torch.Tensor) else v for k, v in kw.items()}
+    tok, lp = check_sample(S, few, u, **kw)
+    t, p = S.sample_rows(few[i], u[i], **big)
+    assert torch.equal(t, tok[i]) and torch.equal(p, lp[i])
+
+
+def test_sample_step_of_many_rows(S):
+    """The decoder's bookkeeping behind the first piece of a batch."""
+    import ctypes as C
+    from ecog2txt_amd import hip_lib as H
+    V, L, eos, pad = 16378, 3, 1, 0
+    n, B = 37, 65535 + 45
+    i = torch.arange(B, device='cuda') % n
+    few, u = (torch.randn(n, V, generator=gen(1), device='cuda') * 2).bfloat16(), torch.rand(n, generator=gen(2), device='cuda')
+    few[5, eos] = 90.0
+    got = []
+    for l, v in ((few, u), (few[i], u[i])):
+        b = len(v)
+        temp = (0.5 + torch.arange(n, device='cuda') / n)[torch.arange(b, device='cuda') % n].contiguous()
+        done = (torch.arange(b, device='cuda') % n == 9).int()
+        out, nxt, score = (torch.full(s, -5, dtype=d, device='cuda') for s, d in (((b, L), torch.int32), ((b,), torch.int32), ((b,), torch.float32)))
+        cfg = S.sample_config(b, l.get_device(), temperature=temp, top_k=30)
+        need = H.lib.e2t_sample_ws_bytes(b, V)
+        ws = torch.empty(need, dtype=torch.uint8, device='cuda')
+        H.lib.e2t_sample_step(l.data_ptr(), H.DT_BF16, V, b, V, v.data_ptr(), C.byref(cfg), 1, L, eos, pad, done.data_ptr(), out.data_ptr(), nxt.data_ptr(),
+                              score.data_ptr(), ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        got.append((done, out, nxt, score))
+    for one, many in zip(*got):
+        assert torch.equal(one[i], many)
+    assert got[0][0][5] == 1 and got[0][1][9, 1] == pad and got[0][3][9] == -5 and (got[0][1][:, [0, 2]] == -5).all()

@@ -23,3 +23,11 @@ def test_negated_views():
     assert x.is_neg()
     with pytest.raises(ValueError, match='resolve_neg'):
         S.quantize_rows(x)
+
+
+def test_workspace_of_a_batch_in_pieces():
+    from ecog2txt_amd.hip_lib import lib
+    n = lib.e2t_sample_ws_bytes(65535, 20000)
+    assert n and lib.e2t_sample_ws_bytes(65536, 20000) == n == lib.e2t_sample_ws_bytes(2 ** 31 - 1, 20000)
+    assert lib.e2t_sample_ws_bytes(65534, 20000) < n
+    assert lib.e2t_sample_ws_bytes(2 ** 31 - 1, 16377) == 0 == lib.e2t_sample_ws_bytes(3, 1048577)
