@@ -93,7 +93,8 @@ int64_t rows_stride(PyObject* q, PyObject* scale, int64_t cols) {
     if (cols <= 0 || cols > E2T_I8_MAX_ROWS || (cols + 63) / 64 * 64 > m.cols)
         bad("q needs %lld columns (the %lld of the matrix, rounded up to 64)", (long long)(cols + 63) / 64 * 64, (long long)cols);
     if (cols > E2T_I8_MAX_K) bad("more than %d columns overflow the 32-bit sums", E2T_I8_MAX_K);
-    if (m.rows <= 1) m.ld = m.cols / 64 * 64;
+    if (m.rows <= 1) m.ld = (cols + 63) / 64 * 64;
+    if (m.ld > E2T_I8_MAX_LD) bad("rows of q lie more than %d bytes apart", E2T_I8_MAX_LD);
     if (((uintptr_t)m.t->data_ptr() | (uintptr_t)m.ld) & 15) bad("the rows of q must start on 16-byte boundaries");
     vector(scale, m.rows, at::kFloat, m.dev, "scale");
     return m.ld;
@@ -167,6 +168,7 @@ E2T_PY(check_rows, 3) {
 // quantize(x) -> q, scale
 E2T_PY(quantize, 1) {
     const Mat x = matrix(a[0], "x", at::kFloat, at::kBFloat16);
+    if (x.cols > E2T_I8_MAX_K) bad("more than %d columns overflow the 32-bit sums", E2T_I8_MAX_K);
     const at::Tensor q = fresh(*x.t, {x.rows, (x.cols + 63) / 64 * 64}, at::kChar), scale = fresh(*x.t, {x.rows}, at::kFloat);
     if (x.rows)
         call("e2t_quant_rows_i8", x.dev, e2t_quant_rows_i8_p, x.t->data_ptr(), dt_of(*x.t), (long long)x.ld, (int)x.rows, (int)x.cols, (int8_t*)q.data_ptr(),
@@ -200,6 +202,7 @@ E2T_PY(linear, 6) {
 // sample(logits, u, temperature, top_k, top_p, min_p) -> token, logprob
 E2T_PY(sample, 6) {
     const Mat l = matrix(a[0], "logits", at::kFloat, at::kBFloat16);
+    if (l.cols > E2T_SAMPLE_MAX_V) bad("more than %d logits a row", E2T_SAMPLE_MAX_V);
     const float* u = (const float*)vector(a[1], l.rows, at::kFloat, l.dev, "u");
     e2t_sample_cfg c{};
     auto number = [&](PyObject* v, const char* name, float& all, const float*& rows) {

@@ -192,3 +192,23 @@ def test_sample_step_of_many_rows(S):
     for one, many in zip(*got):
         assert torch.equal(one[i], many)
     assert got[0][0][5] == 1 and got[0][1][9, 1] == pad and got[0][3][9] == -5 and (got[0][1][:, [0, 2]] == -5).all()
+
+
+def test_limits_of_sizes_are_value_errors(S):
+    ones = torch.ones(3, device='cuda')
+    with pytest.raises(ValueError, match='1048576'):
+        S.sample_rows(torch.zeros(3, 1048577, dtype=torch.bfloat16, device='cuda'), ones / 2)
+    with pytest.raises(ValueError, match='131071'):
+        S.quantize_rows(torch.zeros(1, 131072, device='cuda'))
+    store = torch.zeros(2 * 8388624 + 128, dtype=torch.int8, device='cuda')
+    with pytest.raises(ValueError, match='8388608'):
+        S.Int8Rows(store.as_strided((3, 128), (8388624, 1)), ones, 100)
+    # the furthest rows that are served, and one row of any width
+    far = store.as_strided((3, 128), (8388608, 1))
+    far[:, :100] = torch.randint(-127, 128, (3, 100), generator=gen(1), device='cuda', dtype=torch.int32).to(torch.int8)
+    w = S.quantize_rows(torch.randn(20, 100, generator=gen(2), device='cuda'))
+    near = far.contiguous()
+    assert torch.equal(S.matmul_i8(S.Int8Rows(far, ones, 100), w), S.matmul_i8(S.Int8Rows(near, ones, 100), w))
+    assert torch.equal(S.matmul_i8(w, S.Int8Rows(far, ones, 100)), S.matmul_i8(w, S.Int8Rows(near, ones, 100)))
+    row = store[None, :store.numel() // 64 * 64]
+    assert torch.equal(S.matmul_i8(S.Int8Rows(row, ones[:1], 100), w), S.matmul_i8(S.Int8Rows(near[:1], ones[:1], 100), w))
