@@ -412,7 +412,7 @@ template <int BM, int BN, int WM, int WN, int NS, int KS, int WGS, bool QUARTERS
     constexpr int lds = (BM + BN) * 64 * NS * KS + (BM + 2 * BN) * 4;
     static_assert(lds * WGS <= 160 * 1024, "LDS");
     const long long W = (long long)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
-    E2T_CHECK_ARG(W < (1ll << 29));
+    E2T_CHECK_ARG(W < (1ll << 24));
     p.full = (int)W;
     if (QUARTERS) { const int left = (int)(W % 256); if (W > 256 && left <= I8_QUARTERED) p.full = (int)W - left; }
     const unsigned grid = (unsigned)(p.full + (W - p.full) * 4);
@@ -491,21 +491,31 @@ template <int NTL, int NWV, int D> static int i8_fused_launch(const I8Args& p, v
     E2T_LAUNCH_CHECK(); return E2T_OK;
 }
 
+// A launch has fewer than 2^32 threads.  What needs more runs in pieces: rows to quantise (256 threads each at most), columns of a product (at
+// most 512 threads for sixteen), and as many of its rows as then make fewer than 2^24 tiles of 64 x 64 (256 threads each).
+#define I8_QUANT_ROWS (1 << 22)
+#define I8_COLS (1 << 20)
 extern "C" int e2t_quant_rows_i8(const void* x, int dtype, long long ldx, int M, int K, int8_t* q, long long ldq, float* scale, void* stream) {
     E2T_CHECK_ARG(x && q && scale && M > 0 && M <= E2T_I8_MAX_ROWS && K > 0 && K < (1 << 30) && ldx >= K && (dtype == E2T_DT_F32 || dtype == E2T_DT_BF16));
     E2T_CHECK_ARG(ldq >= ((K + 63) & ~63) && (ldq & 15) == 0 && ((uintptr_t)q & 15) == 0 && ((uintptr_t)x & (dtype == E2T_DT_F32 ? 3 : 1)) == 0);
     const int vec = (((uintptr_t)x | (unsigned long long)(ldx * (dtype == E2T_DT_F32 ? 4 : 2))) & 15) == 0;
 #define QL(T, NC)                                                                                                                             \
     do {                                                                                                                                      \
-        const dim3 g((M + 256 / T - 1) / (256 / T));                                                                                          \
-        if (dtype == E2T_DT_BF16) hipLaunchKernelGGL((k_quant_rows<true, T, NC>), g, dim3(256), 0, ST, x, ldx, M, K, vec, q, ldq, scale);       \
-        else hipLaunchKernelGGL((k_quant_rows<false, T, NC>), g, dim3(256), 0, ST, x, ldx, M, K, vec, q, ldq, scale);                           \
+        const dim3 g((rows + 256 / T - 1) / (256 / T));                                                                                       \
+        if (dtype == E2T_DT_BF16) hipLaunchKernelGGL((k_quant_rows<true, T, NC>), g, dim3(256), 0, ST, xs, ldx, rows, K, vec, qs, ldq, scale + m0);  \
+        else hipLaunchKernelGGL((k_quant_rows<false, T, NC>), g, dim3(256), 0, ST, xs, ldx, rows, K, vec, qs, ldq, scale + m0);                      \
     } while (0)
-    if (K <= 1024 && M >= 512) QL(64, 2);
-    else if (K <= 4096) QL(256, 2);
-    else QL(256, 4);
+    for (int m0 = 0; m0 < M; m0 += I8_QUANT_ROWS) {
+        const int rows = M - m0 < I8_QUANT_ROWS ? M - m0 : I8_QUANT_ROWS;
+        const void* xs = (const char*)x + (size_t)m0 * ldx * (dtype == E2T_DT_F32 ? 4 : 2);
+        int8_t* qs = q + (size_t)m0 * ldq;
+        if (K <= 1024 && M >= 512) QL(64, 2);
+        else if (K <= 4096) QL(256, 2);
+        else QL(256, 4);
+        E2T_LAUNCH_CHECK();
+    }
 #undef QL
-    E2T_LAUNCH_CHECK(); return E2T_OK;
+    return E2T_OK;
 }
 
 static int gemm_i8_check(const void* B, long long ldb, const float* sb, const void* C, long long ldc, int M, int N, int K, int flags) {
@@ -527,9 +537,18 @@ extern "C" int e2t_gemm_nt_i8(const int8_t* A, long long lda, const float* sa, c
                               const float* bias, void* C, long long ldc, int M, int N, int K, int flags, void* stream) {
     if (int rc = gemm_i8_check(B, ldb, sb, C, ldc, M, N, K, flags)) return rc;
     E2T_CHECK_ARG(A && sa && lda <= E2T_I8_MAX_LD && lda >= (((long long)K + 63) & ~63ll) && (lda & 15) == 0 && ((uintptr_t)A & 15) == 0);
-    I8Args p = i8_args(B, ldb, sb, bias, C, ldc, M, N, K, flags);
-    p.A = A; p.sa = sa; p.lda = lda;
-    return i8_launch(p, stream);
+    const int nn = N < I8_COLS ? N : I8_COLS;
+    const long long fit = (((1ll << 24) / ((nn + 63) / 64) - 1) * 64) & ~255ll;
+    const int mm = M < fit ? M : (int)fit;
+    const size_t es = flags & E2T_GEMM_OUT_BF16 ? 2 : 4;
+    for (int n0 = 0; n0 < N; n0 += nn)
+        for (long long m0 = 0; m0 < M; m0 += mm) {
+            I8Args p = i8_args(B + (size_t)n0 * ldb, ldb, sb + n0, bias ? bias + n0 : nullptr, (char*)C + ((size_t)m0 * ldc + n0) * es, ldc,
+                               M - m0 < mm ? (int)(M - m0) : mm, N - n0 < nn ? N - n0 : nn, K, flags);
+            p.A = A + (size_t)m0 * lda; p.sa = sa + m0; p.lda = lda;
+            if (int rc = i8_launch(p, stream)) return rc;
+        }
+    return E2T_OK;
 }
 
 extern "C" int e2t_gemm_i8_instance(int M, int N, int K) {
@@ -553,9 +572,13 @@ extern "C" int e2t_linear_i8(const void* x, int dtype, long long ldx, const int8
     E2T_CHECK_ARG((ws || lin_fused(M, N, K)) && ws_bytes >= e2t_linear_i8_ws_bytes(M, N, K) && ((uintptr_t)ws & 15) == 0);
     E2T_CHECK_ARG(x && ldx >= K && (dtype == E2T_DT_F32 || dtype == E2T_DT_BF16) && ((uintptr_t)x & (dtype == E2T_DT_F32 ? 3 : 1)) == 0);
     if (lin_fused(M, N, K)) {
-        I8Args p = i8_args(W, ldw, sw, bias, y, ldy, M, N, K, flags);
-        p.x = x; p.ldx = ldx; p.xbf16 = dtype == E2T_DT_BF16; p.xvec = (((uintptr_t)x | (unsigned long long)(ldx * (p.xbf16 ? 2 : 4))) & 15) == 0;
-        return i8_fused_launch<1, 8, 4>(p, stream);
+        for (int n0 = 0; n0 < N; n0 += I8_COLS) {
+            I8Args p = i8_args(W + (size_t)n0 * ldw, ldw, sw + n0, bias ? bias + n0 : nullptr, (char*)y + n0 * (size_t)(flags & E2T_GEMM_OUT_BF16 ? 2 : 4), ldy, M,
+                               N - n0 < I8_COLS ? N - n0 : I8_COLS, K, flags);
+            p.x = x; p.ldx = ldx; p.xbf16 = dtype == E2T_DT_BF16; p.xvec = (((uintptr_t)x | (unsigned long long)(ldx * (p.xbf16 ? 2 : 4))) & 15) == 0;
+            if (int rc = i8_fused_launch<1, 8, 4>(p, stream)) return rc;
+        }
+        return E2T_OK;
     }
     const long long ldq = (K + 63) & ~63;
     float* sx = (float*)((char*)ws + lin_q_bytes(M, K));

@@ -338,7 +338,7 @@ int e2t_quant_rows_i8(const void* x, int dtype, long long ldx, int M, int K, int
 #define E2T_I8_MAX_LD 8388608       /* largest lda / ldb: a tile's rows are addressed with 32 bits */
 int e2t_gemm_nt_i8(const int8_t* A, long long lda, const float* sa, const int8_t* B, long long ldb, const float* sb, const float* bias,
                    void* C, long long ldc, int M, int N, int K, int flags, void* stream);
-/* which of the product's instances these sizes run on, 0 .. 10 (-1: sizes that are refused): the sums are the same on all of them; for
+/* which of the product's instances these sizes run on (below 2^20 columns and 2^24 tiles of 64 x 64, where one launch does it), 0 .. 10 (-1: sizes that are refused): the sums are the same on all of them; for
  * tests, which have to reach each */
 int e2t_gemm_i8_instance(int M, int N, int K);
 /* the same from activations: e2t_quant_rows_i8(x) and e2t_gemm_nt_i8 in one call.  ws: device memory of e2t_linear_i8_ws_bytes(M, N, K),

@@ -212,3 +212,56 @@ def test_limits_of_sizes_are_value_errors(S):
     assert torch.equal(S.matmul_i8(w, S.Int8Rows(far, ones, 100)), S.matmul_i8(w, S.Int8Rows(near, ones, 100)))
     row = store[None, :store.numel() // 64 * 64]
     assert torch.equal(S.matmul_i8(S.Int8Rows(row, ones[:1], 100), w), S.matmul_i8(S.Int8Rows(near[:1], ones[:1], 100), w))
+
+
+# ---------------------------------------------------------------------------------------------------- more rows or columns than one launch has
+def free_bytes(n):
+    torch.cuda.empty_cache()
+    return torch.cuda.mem_get_info()[0] > n
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('M,K', [((1 << 26) + 5, 3), ((1 << 22) + 9, 1030)])
+def test_quantize_rows_of_any_number(S, M, K, dtype):
+    if not free_bytes(M * (K + 63) // 64 * 64 + 3 * M * K * 4):
+        pytest.skip('not enough free memory')
+    x = torch.randn(M, K, generator=gen(K), device='cuda').to(dtype)
+    r = S.quantize_rows(x)
+    step = 1 << 20
+    for a in list(range(0, M, step * 8)) + [M - step]:
+        part = S.quantize_rows(x[a:a + step])
+        assert torch.equal(part.q, r.q[a:a + step]) and torch.equal(part.scale, r.scale[a:a + step])
+    if K < 8:                                                          # and as rows of a product
+        w = S.quantize_rows(torch.randn(2, K, generator=gen(1), device='cuda'))
+        y = S.matmul_i8(r, w)
+        for a in (0, 1 << 25, M - 4000):
+            assert torch.equal(y[a:a + 4000], S.matmul_i8(S.Int8Rows(r.q[a:a + 4000], r.scale[a:a + 4000], K), w))
+
+
+def test_product_and_layer_of_any_number_of_columns(S):
+    N, K = (1 << 28) + 48, 5
+    if not free_bytes(N * 64 + 12 * N * 4):
+        pytest.skip('not enough free memory')
+    q = torch.zeros(N, 64, dtype=torch.int8, device='cuda')
+    q[:, :K] = torch.randint(-127, 128, (N, K), generator=gen(1), device='cuda', dtype=torch.int8)
+    w = S.Int8Rows(q, torch.ones(N, device='cuda'), K)
+    x = torch.randint(-126, 127, (1, K), generator=gen(2), device='cuda').float()
+    x[0, 2] = 127                                                      # (its scale is 1: the quantised row is the row)
+    bias = torch.arange(N, device='cuda').remainder(17).float()
+    want = (q[:, :K].float() * x).sum(1) + bias                        # (whole numbers below 2^24: exact)
+    a = S.quantize_rows(x)
+    assert a.scale[0] == 1
+    assert torch.equal(S.matmul_i8(a, w, bias=bias)[0], want)
+    assert torch.equal(S.linear_i8(x, w, bias=bias)[0], want)
+    assert torch.equal(S.linear_i8(x, w, bias=bias, out_dtype=torch.bfloat16)[0], want.bfloat16())
+
+
+def test_product_of_any_number_of_tiles(S):
+    M, N, K = (1 << 18) + 100, 1 << 18, 4
+    if not free_bytes(M * N * 2 + (8 << 30)):
+        pytest.skip('not enough free memory')
+    a, w = (S.quantize_rows(torch.randn(n, K, generator=gen(n % 7), device='cuda')) for n in (M, N))
+    y = S.matmul_i8(a, w, out_dtype=torch.bfloat16)
+    rows = torch.cat([torch.arange(i, i + 64) for i in (0, 65200, 65280, 131000, 262048, 262080, M - 64)] + [torch.randint(M, (300,))]).cuda()
+    for i in rows.split(64):
+        assert torch.equal(y[i], S.matmul_i8(S.Int8Rows(a.q[i], a.scale[i], K), w, out_dtype=torch.bfloat16))
