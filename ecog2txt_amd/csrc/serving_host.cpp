@@ -36,10 +36,11 @@ const char* type_name(at::ScalarType t) { return t == at::kFloat ? "float32" : t
 // nothing here has a gradient: a tensor that asks for one, in reverse or in forward mode, is refused; and memory is read as it lies, so
 // that a view which stands for its negative (the imaginary part of a conjugate) is refused, too
 void plain(const at::Tensor& t, const char* name) {
+    if (t.is_neg()) bad("%s is a view of the negative of what its memory holds (use its resolve_neg())", name);
+    if (!t.unsafeGetTensorImpl()->autograd_meta()) return;       // (most have none: spares three calls into torch)
     if (t.requires_grad() && at::GradMode::is_enabled()) bad("%s asks for a gradient: the serving operators have none (use torch.no_grad())", name);
     if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
         bad("%s has a forward-mode tangent: the serving operators pass none on", name);
-    if (t.is_neg()) bad("%s is a view of the negative of what its memory holds (use its resolve_neg())", name);
 }
 struct Mat { const at::Tensor* t; int64_t rows, cols, ld; int dev; };
 // a 2-D device tensor with contiguous rows
@@ -87,44 +88,43 @@ template <class F, class... A> void call(const char* name, int dev, F f, A... a)
     if (rc) { PyErr_Format(PyExc_RuntimeError, "%s failed (%d): %s", name, rc, e2t_last_error_p()); throw Bad(); }
 }
 
-// q and scale of a matrix in 8 bits with `cols` columns: its row stride
-int64_t rows_stride(PyObject* q, PyObject* scale, int64_t cols) {
-    Mat m = matrix(q, "q", at::kChar, at::kChar);
-    if (cols <= 0 || cols > E2T_I8_MAX_ROWS || (cols + 63) / 64 * 64 > m.cols)
-        bad("q needs %lld columns (the %lld of the matrix, rounded up to 64)", (long long)(cols + 63) / 64 * 64, (long long)cols);
+// a matrix in 8 bits with `cols` columns
+struct RowsMem { const at::Tensor* t; int64_t n, ld; int dev; const int8_t* q; const float* scale; };
+RowsMem rows_mem(PyObject* q, PyObject* scale, int64_t cols) {
+    const Mat m = matrix(q, "q", at::kChar, at::kChar);
+    const int64_t cols64 = (cols + 63) / 64 * 64;
+    if (cols <= 0 || cols > E2T_I8_MAX_ROWS || cols64 > m.cols) bad("q needs %lld columns (the %lld of the matrix, rounded up to 64)", (long long)cols64, (long long)cols);
     if (cols > E2T_I8_MAX_K) bad("more than %d columns overflow the 32-bit sums", E2T_I8_MAX_K);
-    if (m.rows <= 1) m.ld = (cols + 63) / 64 * 64;
-    if (m.ld > E2T_I8_MAX_LD) bad("rows of q lie more than %d bytes apart", E2T_I8_MAX_LD);
-    if (((uintptr_t)m.t->data_ptr() | (uintptr_t)m.ld) & 15) bad("the rows of q must start on 16-byte boundaries");
-    vector(scale, m.rows, at::kFloat, m.dev, "scale");
-    return m.ld;
+    RowsMem r{m.t, m.rows, m.rows <= 1 ? cols64 : m.ld, m.dev, (const int8_t*)m.t->data_ptr(), nullptr};
+    if (r.ld > E2T_I8_MAX_LD) bad("rows of q lie more than %d bytes apart", E2T_I8_MAX_LD);
+    if (((uintptr_t)r.q | (uintptr_t)r.ld) & 15) bad("the rows of q must start on 16-byte boundaries");
+    r.scale = (const float*)vector(scale, m.rows, at::kFloat, m.dev, "scale");
+    return r;
 }
 // an Int8Rows, by its attributes, which may have been set (or their tensors resized) since it was made: they are checked in every call
-struct Rows {
-    THPObjectPtr q, scale;
-    int64_t cols = 0, ld = 0;
+struct Rows : RowsMem {
+    THPObjectPtr hold_q, hold_scale;
+    int64_t cols = 0;
     explicit Rows(PyObject* o, const char* name) {
         const int is = PyObject_IsInstance(o, rows_type);
         if (is < 0) throw Bad();
         if (!is) bad("%s must be Int8Rows", name);
         THPObjectPtr c(PyObject_GetAttr(o, s_cols));
-        q = PyObject_GetAttr(o, s_q); scale = PyObject_GetAttr(o, s_scale);
-        if (!c || !q || !scale) throw Bad();
+        hold_q = PyObject_GetAttr(o, s_q); hold_scale = PyObject_GetAttr(o, s_scale);
+        if (!c || !hold_q || !hold_scale) throw Bad();
         cols = PyLong_AsLongLong(c.get());
         if (cols == -1 && PyErr_Occurred()) throw Bad();
-        ld = rows_stride(q.get(), scale.get(), cols);
+        *(RowsMem*)this = rows_mem(hold_q.get(), hold_scale.get(), cols);
     }
-    const at::Tensor& qt() { return THPVariable_Unpack(q.get()); }
-    const float* sp() { return (const float*)THPVariable_Unpack(scale.get()).data_ptr(); }
 };
 struct Out { at::Tensor made; const at::Tensor* t; int64_t n, ld; const float* bias; int flags; };
 // weights, bias, output type and output of a product with `rows` rows of activations
-Out output(Rows& w, int64_t cols, PyObject* bias, PyObject* out_dtype, PyObject* relu, PyObject* out, int64_t rows, const at::Tensor& like) {
+Out output(const Rows& w, int64_t cols, PyObject* bias, PyObject* out_dtype, PyObject* relu, PyObject* out, int64_t rows, const at::Tensor& like) {
     const int dev = like.get_device();
-    if (w.qt().get_device() != dev) bad("the weights must be Int8Rows on device %d", dev);
+    if (w.dev != dev) bad("the weights must be Int8Rows on device %d", dev);
     if (w.cols != cols) bad("%lld columns of activations, %lld of weights", (long long)cols, (long long)w.cols);
     Out o{};
-    o.n = w.qt().size(0);
+    o.n = w.n;
     if (o.n == 0) bad("the weights have no rows");
     const at::ScalarType type = THPDtype_Check(out_dtype) ? ((THPDtype*)out_dtype)->scalar_type : at::kByte;
     if (type != at::kFloat && type != at::kBFloat16) bad("out_dtype must be float32 or bfloat16");
@@ -163,7 +163,7 @@ PyObject* bind(PyObject*, PyObject* const*, Py_ssize_t);
 E2T_PY(check_rows, 3) {
     const int64_t cols = PyLong_AsLongLong(a[2]);
     if (cols == -1 && PyErr_Occurred()) throw Bad();
-    return PyLong_FromLongLong(rows_stride(a[0], a[1], cols));
+    return PyLong_FromLongLong(rows_mem(a[0], a[1], cols).ld);
 }
 // quantize(x) -> q, scale
 E2T_PY(quantize, 1) {
@@ -177,24 +177,23 @@ E2T_PY(quantize, 1) {
 }
 // matmul(a, w, bias, out_dtype, relu, out) -> out
 E2T_PY(matmul, 6) {
-    Rows x(a[0], "a"), w(a[1], "w");
-    const at::Tensor& q = x.qt();
-    const Out o = output(w, x.cols, a[2], a[3], a[4], a[5], q.size(0), q);
-    if (q.size(0))
-        call("e2t_gemm_nt_i8", q.get_device(), e2t_gemm_nt_i8_p, (const int8_t*)q.data_ptr(), (long long)x.ld, x.sp(), (const int8_t*)w.qt().data_ptr(), (long long)w.ld,
-             w.sp(), o.bias, o.t->data_ptr(), (long long)o.ld, (int)q.size(0), (int)o.n, (int)x.cols, o.flags);
+    const Rows x(a[0], "a"), w(a[1], "w");
+    const Out o = output(w, x.cols, a[2], a[3], a[4], a[5], x.n, *x.t);
+    if (x.n)
+        call("e2t_gemm_nt_i8", x.dev, e2t_gemm_nt_i8_p, x.q, (long long)x.ld, x.scale, w.q, (long long)w.ld, w.scale, o.bias, o.t->data_ptr(), (long long)o.ld, (int)x.n,
+             (int)o.n, (int)x.cols, o.flags);
     return wrap(o, a[5]);
 }
 // linear(x, w, bias, out_dtype, relu, out) -> out
 E2T_PY(linear, 6) {
     const Mat x = matrix(a[0], "x", at::kFloat, at::kBFloat16);
-    Rows w(a[1], "w");
+    const Rows w(a[1], "w");
     const Out o = output(w, x.cols, a[2], a[3], a[4], a[5], x.rows, *x.t);
     if (x.rows) {
         const size_t need = e2t_linear_i8_ws_bytes_p((int)x.rows, (int)o.n, (int)x.cols);
         at::Tensor ws;
         if (need) ws = fresh(*x.t, {(int64_t)need}, at::kByte);
-        call("e2t_linear_i8", x.dev, e2t_linear_i8_p, x.t->data_ptr(), dt_of(*x.t), (long long)x.ld, (const int8_t*)w.qt().data_ptr(), (long long)w.ld, w.sp(), o.bias,
+        call("e2t_linear_i8", x.dev, e2t_linear_i8_p, x.t->data_ptr(), dt_of(*x.t), (long long)x.ld, w.q, (long long)w.ld, w.scale, o.bias,
              o.t->data_ptr(), (long long)o.ld, (int)x.rows, (int)o.n, (int)x.cols, o.flags, need ? ws.data_ptr() : nullptr, need);
     }
     return wrap(o, a[5]);
