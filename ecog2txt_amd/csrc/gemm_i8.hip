@@ -56,8 +56,8 @@ __device__ __forceinline__ uint2 quant8(const f8& x, float top, float inv) {
 }
 
 // Rows to 8 bits: T threads a row, NC groups of eight elements a thread in registers between the maximum and the rounding (longer rows
-// come from the cache a second time).  Bound by its bytes: fp32 4099 x 4104 in 18.7 us = 4.5 TB/s, what a large copy reaches
-// (4.7).
+// come from the cache a second time).  Bound by its bytes: fp32 4099 x 4104 from memory in 20.7 us = 4.1 TB/s (a large copy 4.7, a large
+// read 4.0).
 template <bool BF16, int T, int NC> __global__ __launch_bounds__(256) void k_quant_rows(const void* x, long long ldx, int M, int K, int vec, int8_t* q,
                                                                                        long long ldq, float* scale) {
     __shared__ float red[4];
@@ -234,7 +234,7 @@ __device__ __forceinline__ void i8_tile(const I8Args& p, int m0, int n0) {
         const size_t cs = (size_t)p.ldc * es;
         const int nb = ncols * es;                         // bytes of a row
         // as many bytes a lane as the rows' alignment allows; all of the wave's rows are read before the first is stored (with a loop in which each
-        // store waited for its own LDS read, 7398 x 4337 x 812 took 70 us by elements, so 53; in whole 16 bytes (4336) 49, so 45)
+        // store waited for its own LDS read, 7398 x 4337 x 812 took 70 us by elements, so 51; in whole 16 bytes (4336) 49, so 45)
         auto put = [&](auto type, auto places) {
             using T = decltype(type);
             constexpr int PER = decltype(places)::value, RPI = 64 / PER, N = 16 / RPI;          // places of a row, rows an instruction
@@ -267,7 +267,9 @@ __device__ __forceinline__ int xcd_order(int L, int W) {
     return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + idx;
 }
 // tile w of ntm x ntn, in blocks of eight tile rows: the tiles an XCD has in flight (32 of 256 x 256) share few panels of either operand
-// (8192^3: 522 us in columns of the whole height, 481 in blocks: the panels then stay in the XCD's 4 MB of L2)
+// (8192^3: 475 us in columns of the whole height, 446 in blocks; 8704 x 8192 x 2048 166 and 157: the panels then stay in the XCD's 4 MB of L2.
+// Where a dimension ends just behind a tile its edge strips count like whole tiles: 4099 x 4100 has 17 x 17, of which eight strips go into
+// the full round and eight whole tiles into the quartered rest)
 __device__ __forceinline__ void tile_of(int w, int ntm, int ntn, int& tm, int& tn) {
     constexpr int GM = 8;
     const int g = w / (GM * ntn), gr = min(GM, ntm - g * GM), o = w - g * GM * ntn;
@@ -433,10 +435,12 @@ template <int MT, int NTL, int NWV, int D> static int i8_rows_launch(const I8Arg
     E2T_LAUNCH_CHECK(); return E2T_OK;
 }
 // Which instance: the one whose predicted time is the shortest.  The predictions (microseconds; S = 64-byte k-blocks, W = tiles) are straight
-// lines through measured times of every instance at 120 shapes, M 16 .. 8704, N 100 .. 16384, K 64 .. 16384; over 110 other shapes, M from 1,
-// the chosen instance takes 3 % more than the best one on average and 30 % at most.  Both sides of the larger steps:
-//   M = 16, 4096 x 4096: rows 5.7, 64 x 64 tiles 14.3;   M = 128: rows 12.9, tiles in two K groups 13.0;   M = 256: rows 18.9, tiles 13.5
-//   M = 1024, 4096 x 4096: 64 x 64 39, 128 x 128 31, 128 x 128 in two K groups 26, 256 x 256 51;   M = 4096: 128 x 128 89, 256 x 256 63
+// lines through measured times of every instance at 120 shapes, M 16 .. 8704, N 100 .. 16384, K 64 .. 16384.  The chosen instance takes 3 % more
+// than the best one on average, there and over 110 other shapes (M from 1); on those it is 29 % off at most, on the fitted ones 51 % at
+// 512 x 512 x 16384 (30.1 us, 20.0), 32 % at 501 x 347 x 13543 and 20 % elsewhere.  Both sides of the larger steps:
+//   M = 16, 4096 x 4096: rows 4.8, 64 x 64 tiles 13.8;   M = 128: rows 11.2, tiles in two K groups 12.0;   M = 256: rows 20.6, tiles 12.5
+//   M = 1024, 4096 x 4096: 64 x 64 41, 128 x 128 31, 128 x 128 in two K groups 27, 256 x 256 52;   M = 4096: 128 x 128 84, 256 x 256 63
+// No instance splits K over workgroups: few tiles of a long K take two to ten times their floor (464 x 4103 x 11997 58 us, floor 21).
 static int i8_instance(int M, int N, int K) {
     const double S = (K + 63) / 64, K64 = 64.0 * S, bytes = N * K64;
     auto cdiv = [](long long a, long long b) { return (double)((a + b - 1) / b); };
@@ -556,9 +560,11 @@ extern "C" int e2t_gemm_i8_instance(int M, int N, int K) {
 }
 
 static inline size_t lin_q_bytes(int M, int K) { return ((size_t)M * (size_t)((K + 63) & ~63) + 255) & ~(size_t)255; }
-// One launch where quantising again in every workgroup (16 outputs each) costs less than a launch of its own: N = 1806 .. 4096, us for one / two
-// launches: M = 1, K = 4096 5.5 / 8.0; M = 2, K = 8192 10.8 / 12; M = 4, K = 2048 6.2 / 6.5, K = 4096 9.4 / 8.5; M = 8, K = 1024 5.8 / 6.0; M = 13,
-// K = 624 8.5 / 6.2.  Many outputs: N = 9000, M = 1, K = 2048 6.5 / 7.5; N = 16384 9.6 / 9.0, K = 4096 14.6 / 16.0; M = 2 18 / 16.
+// One launch where quantising again in every workgroup (16 outputs each) costs less than a launch of its own.  us for one / two launches,
+// N = 1806 .. 4096: M = 1, K = 4096 5.2 / 7.8; M = 2, K = 8192 10 / 12; M = 4, K = 2048 6.0 / 6.4, K = 4096 9.1 / 8.3; M = 8, K = 1024 5.6 / 6.2,
+// K = 2048 8.3 / 6.6.  Many outputs: N = 9000, M = 1, K = 2048 6.1 / 7.6, M = 2 6.9 / 7.8, M = 4 8.4 / 7.8; N = 16384, M = 1, K = 4096 12.6 / 16.2,
+// M = 2 17.5 / 16.2.  (In one launch M = 1 gains at every N measured: above 12288 outputs and below K = 4096 the rule still takes two, 9.0 us for
+// 7.6 at 16384 x 2048.)
 static bool lin_fused(int M, int N, int K) {
     if ((size_t)M * (((K + 63) & ~63) + 16) > 100 * 1024) return false;
     return N > 8192 ? M == 1 && (K >= 4096 || N <= 12288) : M <= 2 || (M <= 8 && M * K <= 8192);

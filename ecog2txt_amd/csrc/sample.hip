@@ -25,7 +25,7 @@ typedef unsigned long long u64;
 #define SMP_BINS 2048
 #define SMP_TILE 4096               // long rows: tokens of a tile (256 threads x 16)
 #define SMP_CHUNK_TILES 12          // tiles of a workgroup of k_sample_hist at most (the packed word's bits)
-#define SMP_LIST 8192               // long rows: tokens around the cut that are kept in a list
+#define SMP_LIST 8192               // long rows: tokens around the cut that are kept in a list (more: k_sample_draw)
 
 struct SampleArgs {
     const void* logits; long long ldl; int V, frac;            // frac = F
@@ -341,12 +341,15 @@ template <int NT, class Each> __device__ __forceinline__ u64 select_rank(Each ea
 }
 
 // ---- one workgroup a row ---------------------------------------------------------------------------------------------------------------
-// (The histogram here is of 512 or 1024 bins over the row's spread, counts and masses apart: two bins a thread or one, no conversions, and the
-// masses stay in registers for the draw: 1806 tokens with all four settings in 7.2 us, 256 such rows in 8.4.  It is a chain of dependent
-// steps: load 0.7, maximum 0.3, masses and bins 1.3, each cut 1.5, draw and logarithm 1.4.)
+// (The histogram here is of 512 or 1024 bins over the row's spread, counts and masses apart -- masses for top-k alone, too, where the counts would
+// do --: two bins a thread or one, no conversions, and up to 8185 tokens the masses stay in registers for the draw: 1806 tokens with all four
+// settings in 7.2 us, 256 such rows in 8.5.  It is a chain of dependent steps: load 0.7, maximum 0.3, masses and bins 1.3, each cut 1.5, draw
+// and logarithm 1.4.)
 template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sample_row(SampleArgs a) {
     constexpr int E = Row<BF16>::E, NG = VPT / E, NB = VPT <= 8 ? 512 : 1024, PER = NB / NT, NW = NT / 64;
-    constexpr bool HOLD = VPT <= 16;                       // masses in registers (32 of them would spill: they are worked out again)
+    // masses in registers up to 16 tokens a thread; 32 are worked out again where they are needed (that instance takes all 256 registers as it
+    // is, and 44 bytes of scratch a lane)
+    constexpr bool HOLD = VPT <= 16;
     __shared__ u64 red[6 * NW];                            // (a place for each reduction)
     __shared__ ExpTab tab;
     __shared__ u64 hist_m[NB];
@@ -398,7 +401,7 @@ template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sa
     int ci = 0x7FFFFFFF;
     if (st.use_k || st.use_p) {
         short bin[VPT];
-        const double spread = fmin(w.at(-low), (double)SMP_BINS), fine = spread > 0.0 ? 0.999999 * NB / spread : 0.0;      // (a flat row's tokens in few bins: 15 us instead of 7.9)
+        const double spread = fmin(w.at(-low), (double)SMP_BINS), fine = spread > 0.0 ? 0.999999 * NB / spread : 0.0;      // (a flat row's tokens in few bins: 15 us instead of 7.6)
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             const double at = w.at(v[j]);
@@ -472,7 +475,8 @@ template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sa
 // ---- long rows ----------------------------------------------------------------------------------------------------------------------
 // Four launches: k_sample_hist (the row's only whole pass: chunks' histograms, tile maxima), k_sample_zone (which bins hold the cut),
 // k_sample_gather (mass above the cut of every tile that reaches it, and a list of the tokens in the cut's bins), k_sample_draw (the cut, the
-// tile, the token).  Tiles whose maximum lies below the cut are not read again.
+// tile, the token).  Quarter tiles (1024 tokens) whose maximum lies below the cut are not read again; where the kept tokens lie anywhere in the row,
+// 100 of 128003, say, nearly every quarter holds one and the second pass is a whole read, too.
 //
 // A chunk counts before the row's maximum is known (a pass over the logits less): its bins are whole parts of (l - ref) 32 / T from a
 // reference of its own, so they lie across the row's bins floor(32 (z_max - z)).  A token of chunk bin y -- in the row's units -- belongs to
@@ -810,7 +814,10 @@ template <bool BF16> __global__ __launch_bounds__(512) void k_sample_draw(Sample
     u64 cut = ~0ull;
     if (cuts) {
         const u64 above = rec.above, above_c = rec.above_c;
-        // the tokens of the zone: from the list, or, where they are more than it holds (a flat row), from the row itself
+        // the tokens of the zone: from the list, or, where they are more than it holds, from the row itself, by this one workgroup in several
+        // passes (4 x 131072 normal logits of sd 2: 30 us, so 213).  The zone reaches from the first cut to the last and is a sixteenth of a
+        // nat or two wide at least: more than the list are a flat row's tokens, those between a top-p and a far top-k (p 0.5, k 20000), and two
+        // bins of a vocabulary of half a million and more (sd 2, T 1.4, p 0.9: 549 us at 524288, 1058 at 1048576; T 1, p 0.95: 58 and 980)
         auto each = [&](auto f) {
             if (in_list) {
 #pragma unroll
@@ -915,8 +922,8 @@ template <bool BF16> __global__ __launch_bounds__(512) void k_sample_draw(Sample
 }
 
 // ---- entry points -----------------------------------------------------------------------------------------------------------------------
-// (a row may start up to seven elements behind a 16-byte boundary.)  Top-k and top-p in one launch / four: 9000 tokens 20.5 / 27 us, 256 such rows 22 / 35;
-// 15000 21.7 / 28, 23 / 37; half as many in one launch 11 to 12
+// (a row may start up to seven elements behind a 16-byte boundary.)  Top-k and top-p in one launch / four: 9000 tokens 20.3 / 27 us, 256 such rows 22.5 / 35;
+// 15000 20.8 / 28, 24.6 / 37; half as many in one launch 11 to 12
 #define SMP_ROW_MAX (16384 - 7)
 static int frac_bits(int V) { int c = 0; while ((1ll << c) < V) ++c; return 62 - c < 50 ? 62 - c : 50; }
 static int long_tiles(int V) { return (V + 7 + SMP_TILE - 1) / SMP_TILE; }
