@@ -32,7 +32,8 @@ def _bind():
 
 class Int8Rows:
     """A matrix in 8 bits: row i stands for scale[i] * q[i, :cols].  q int8 [rows, >= cols rounded up to 64] (zeros from `cols` up
-    to that), rows 16-byte aligned; scale fp32 [rows]."""
+    to that), rows 16-byte aligned and at most 8388608 bytes apart; scale fp32 [rows].  At most 131071 columns.  (Checked again in every
+    call that it is used in.)"""
     __slots__ = ('q', 'scale', 'cols', 'ld')
 
     def __init__(self, q, scale, cols):
@@ -99,5 +100,5 @@ def sample_config(rows, index, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
 def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """One token for each row of logits [rows, vocabulary] (fp32 or bf16) from one uniform number a row, u fp32 [rows] in [0, 1):
     (token int32 [rows], log-probability among the kept tokens fp32 [rows]).  Settings are numbers or device tensors of one value
-    a row; temperature <= 0 takes the largest logit, top_k <= 0, top_p >= 1 and min_p <= 0 keep everything."""
+    a row; temperature <= 0 takes the largest logit, top_k <= 0, top_p >= 1 and min_p <= 0 keep everything.  At most 1048576 tokens a row, any number of rows."""
     return (_host or _bind()).sample(logits, u, temperature, top_k, top_p, min_p)

@@ -39,7 +39,8 @@ extern "C" {
 int e2t_abi_version(void);
 /* sizeof() of the structs that cross the boundary, for bindings to check their layouts against:
  * which = 0 e2t_gemm_epilogue, 1 e2t_lstm_desc, 2 e2t_pack_desc, 3 e2t_adam_hyper, 4 e2t_dropout, 5 e2t_gemm_call, 6 e2t_tile_desc [ABI 8], 7 e2t_sample_cfg;
- * -1 for any other value */
+ * -1 for any other value.  (The serving entry points joined version 9 without a new number: a library has them where
+ * e2t_sizeof(7) is not -1.) */
 int e2t_sizeof(int which);
 const char* e2t_last_error(void);          /* thread-local, host pointer */
 /* number of compute units / XCDs of `device`, 0 if no device is usable */
