@@ -92,8 +92,8 @@ template <class F, class... A> void call(const char* name, int dev, F f, A... a)
 struct RowsMem { const at::Tensor* t; int64_t n, ld; int dev; const int8_t* q; const float* scale; };
 RowsMem rows_mem(PyObject* q, PyObject* scale, int64_t cols) {
     const Mat m = matrix(q, "q", at::kChar, at::kChar);
-    const int64_t cols64 = (cols + 63) / 64 * 64;
-    if (cols <= 0 || cols > E2T_I8_MAX_ROWS || cols64 > m.cols) bad("q needs %lld columns (the %lld of the matrix, rounded up to 64)", (long long)cols64, (long long)cols);
+    const int64_t cols64 = cols > E2T_I8_MAX_ROWS ? cols : (cols + 63) / 64 * 64;
+    if (cols <= 0 || cols64 > m.cols) bad("q needs %lld columns (the %lld of the matrix, rounded up to 64)", (long long)cols64, (long long)cols);
     if (cols > E2T_I8_MAX_K) bad("more than %d columns overflow the 32-bit sums", E2T_I8_MAX_K);
     RowsMem r{m.t, m.rows, m.rows <= 1 ? cols64 : m.ld, m.dev, (const int8_t*)m.t->data_ptr(), nullptr};
     if (r.ld > E2T_I8_MAX_LD) bad("rows of q lie more than %d bytes apart", E2T_I8_MAX_LD);

@@ -1,12 +1,23 @@
 """What the tensor-level serving calls take, refuse and leave behind: operands changed after they were made, gradients, views that
 are not what memory holds, more rows than one launch has."""
-import numpy as np
 import pytest
 import torch
 
 from test_gpu_serving import check_sample, gen
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def needs():
+    """needs(bytes): skips where the card has not that much; what the test took is given back behind it."""
+    def check(n):
+        torch.cuda.empty_cache()
+        if torch.cuda.mem_get_info()[0] < n:
+            pytest.skip('not enough free memory')
+    yield check
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
 
 
 @pytest.fixture(scope='module')
@@ -155,9 +166,10 @@ def test_sample_rows_of_any_number(S, B, V, dtype):
     check_sample(S, l[-40:], u[-40:], **{n: v[-40:] for n, v in kw.items()})
 
 
-def test_sample_long_rows_of_any_number(S):
+def test_sample_long_rows_of_any_number(S, needs):
     """More long rows than a launch has: copies of a few, each like its original (top-p apart, whose sums depend on the split)."""
     B, V, n = 65535 + 700, 16378, 37
+    needs(16 << 30)
     few, u = (torch.randn(n, V, generator=gen(1), device='cuda') * 2).bfloat16(), torch.rand(n, generator=gen(2), device='cuda')
     kw = dict(settings(n, 3), top_p=1.0)
     i = torch.arange(B, device='cuda') % n
@@ -167,10 +179,11 @@ def test_sample_long_rows_of_any_number(S):
     assert torch.equal(t, tok[i]) and torch.equal(p, lp[i])
 
 
-def test_sample_step_of_many_rows(S):
+def test_sample_step_of_many_rows(S, needs):
     """The decoder's bookkeeping behind the first piece of a batch."""
     import ctypes as C
     from ecog2txt_amd import hip_lib as H
+    needs(16 << 30)
     V, L, eos, pad = 16378, 3, 1, 0
     n, B = 37, 65535 + 45
     i = torch.arange(B, device='cuda') % n
@@ -215,16 +228,10 @@ def test_limits_of_sizes_are_value_errors(S):
 
 
 # ---------------------------------------------------------------------------------------------------- more rows or columns than one launch has
-def free_bytes(n):
-    torch.cuda.empty_cache()
-    return torch.cuda.mem_get_info()[0] > n
-
-
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize('M,K', [((1 << 26) + 5, 3), ((1 << 22) + 9, 1030)])
-def test_quantize_rows_of_any_number(S, M, K, dtype):
-    if not free_bytes(M * (K + 63) // 64 * 64 + 3 * M * K * 4):
-        pytest.skip('not enough free memory')
+def test_quantize_rows_of_any_number(S, M, K, dtype, needs):
+    needs(M * (K + 63) // 64 * 64 + 3 * M * K * 4)
     x = torch.randn(M, K, generator=gen(K), device='cuda').to(dtype)
     r = S.quantize_rows(x)
     step = 1 << 20
@@ -238,10 +245,9 @@ def test_quantize_rows_of_any_number(S, M, K, dtype):
             assert torch.equal(y[a:a + 4000], S.matmul_i8(S.Int8Rows(r.q[a:a + 4000], r.scale[a:a + 4000], K), w))
 
 
-def test_product_and_layer_of_any_number_of_columns(S):
+def test_product_and_layer_of_any_number_of_columns(S, needs):
     N, K = (1 << 28) + 48, 5
-    if not free_bytes(N * 64 + 12 * N * 4):
-        pytest.skip('not enough free memory')
+    needs(N * 64 + 12 * N * 4)
     q = torch.zeros(N, 64, dtype=torch.int8, device='cuda')
     q[:, :K] = torch.randint(-127, 128, (N, K), generator=gen(1), device='cuda', dtype=torch.int8)
     w = S.Int8Rows(q, torch.ones(N, device='cuda'), K)
@@ -256,10 +262,9 @@ def test_product_and_layer_of_any_number_of_columns(S):
     assert torch.equal(S.linear_i8(x, w, bias=bias, out_dtype=torch.bfloat16)[0], want.bfloat16())
 
 
-def test_product_of_any_number_of_tiles(S):
+def test_product_of_any_number_of_tiles(S, needs):
     M, N, K = (1 << 18) + 100, 1 << 18, 4
-    if not free_bytes(M * N * 2 + (8 << 30)):
-        pytest.skip('not enough free memory')
+    needs(M * N * 2 + (8 << 30))
     a, w = (S.quantize_rows(torch.randn(n, K, generator=gen(n % 7), device='cuda')) for n in (M, N))
     y = S.matmul_i8(a, w, out_dtype=torch.bfloat16)
     rows = torch.cat([torch.arange(i, i + 64) for i in (0, 65200, 65280, 131000, 262048, 262080, M - 64)] + [torch.randint(M, (300,))]).cuda()
