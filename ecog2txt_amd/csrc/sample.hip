@@ -473,7 +473,7 @@ template <bool BF16, int NT, int VPT> __global__ __launch_bounds__(NT) void k_sa
 }
 
 // ---- long rows ----------------------------------------------------------------------------------------------------------------------
-// Four launches: k_sample_hist (the row's only whole pass: chunks' histograms, tile maxima), k_sample_zone (which bins hold the cut),
+// Four launches: k_sample_hist (a pass over the whole row: chunks' histograms, tile maxima), k_sample_zone (which bins hold the cut),
 // k_sample_gather (mass above the cut of every tile that reaches it, and a list of the tokens in the cut's bins), k_sample_draw (the cut, the
 // tile, the token).  Quarter tiles (1024 tokens) whose maximum lies below the cut are not read again; where the kept tokens lie anywhere in the row,
 // 100 of 128003, say, nearly every quarter holds one and the second pass is a whole read, too.
